@@ -8,10 +8,11 @@ a multiple of 32 elements, with zeros between them; a step leaves those zeros as
 plain form works on the whole buffer at once and the buffers are what a pass returns.
 
 States in 8 bits: blocks of 32 elements of a tensor share a byte b, the exponent byte of the block's
-largest finite magnitude.  The first moment is sign | e4m3 times 2**(b - 134), the second unsigned
-e5m3 times 2**(b - 127) (table below).  Values are rounded up or down at random, the chance of "up"
-being the distance to the value below: the random number is a function of the tensor's seed, the
-step's count and the element's index.
+largest finite magnitude, but at least 17 (first moment) or 32 (second), so that no code stands for a
+subnormal fp32 number.  The first moment is sign | e4m3 times 2**(b - 134), the second unsigned e5m3
+times 2**(b - 127) (table below).  Values are rounded up or down at random, the chance of "up" being
+the distance to the value below: the random number is a function of the tensor's seed, the step's
+count and the element's index.
 """
 import random
 
@@ -210,7 +211,7 @@ def _encode(x, up, moment):
     blocks = x.abs().view(-1, BLOCK)
     finite = blocks.isfinite()
     largest = torch.where(finite, blocks, 0.0).amax(1)
-    b = (largest.view(torch.int32) >> 23).clamp(8 if moment == 1 else 1, 253)
+    b = (largest.view(torch.int32) >> 23).clamp(17 if moment == 1 else 32, 253)
     y = blocks * _power(254 - b).unsqueeze(1)
     low = -13 if moment == 1 else -28                    # exponent of the smallest normal value
     e = ((y.contiguous().view(torch.int32) >> 23) - 127).clamp(min=low)
@@ -328,8 +329,8 @@ def _exact_rounded(x, chance, moment):
     values = torch.tensor(_exact_codes(moment), dtype=torch.float64, device=x.device)
     mag = x.abs().view(-1, BLOCK)
     _, e = torch.frexp(mag.amax(1, keepdim=True))        # largest = f * 2**e with 0.5 <= f < 1
-    exponent = (e - 1).clamp(-119 if moment == 1 else -126, 126)
-    exponent = torch.where(mag.amax(1, keepdim=True) == 0, -119 if moment == 1 else -126, exponent)
+    exponent = (e - 1).clamp(-110 if moment == 1 else -95, 126)
+    exponent = torch.where(mag.amax(1, keepdim=True) == 0, -110 if moment == 1 else -95, exponent)
     unit = torch.ones_like(mag[:, :1]).ldexp(exponent)
     y = (mag / unit).view(-1)
     below = torch.searchsorted(values, y, right=True) - 1
