@@ -35,6 +35,16 @@ class MuonGroup(ctypes.Structure):
                 ("slots", ctypes.POINTER(c_void_p))]
 
 
+class AdamWGroup(ctypes.Structure):
+    """``fm_adamw_group`` of include/flash_muon_b200.h; the arrays are given by address."""
+    _fields_ = [(name, c_void_p) for name in
+                ("params", "grads", "masters", "exp_avg", "exp_avg_sq", "exp_avg_scale",
+                 "exp_avg_sq_scale", "steps", "numels", "seeds")] + \
+               [(name, ctypes.c_int32) for name in ("count", "p_dtype", "g_dtype", "state_bits")] + \
+               [(name, c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")] + \
+               [("lr_device", c_void_p)]
+
+
 # name -> (restype, argtypes); mirrors include/flash_muon_b200.h one to one
 SIGNATURES = {
     "fm_version": (c_int, []),
@@ -78,6 +88,13 @@ SIGNATURES = {
                                 c_double, c_void_p]),
     "fm_muon_step": (c_int, [ctypes.POINTER(MuonGroup), c_int, ctypes.POINTER(c_void_p),
                              ctypes.c_size_t, c_void_p]),
+    "fm_adamw_step": (c_int, [ctypes.POINTER(AdamWGroup), c_int, c_void_p, c_void_p]),
+    "fm_adamw8_values": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p]),
+    "fm_adamw8_encode": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "fm_grad_norm_workspace_bytes": (c_size_t, [c_int]),
+    "fm_grad_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p,
+                             c_size_t, c_void_p]),
+    "fm_scale_multi": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
 }
 
 

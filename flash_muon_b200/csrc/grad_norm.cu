@@ -1,0 +1,257 @@
+// Norm over all gradients of a model, the factor that clips it, and the scaling by it.  Each is one
+// pass over the gradients: the bound is HBM.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace fm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 8192;         // elements a block takes at a time
+constexpr int kSmallTable = 64;      // tensors of one launch: the table travels as a kernel argument
+constexpr int kLargeTable = 1024;
+constexpr int kMaxBlocks = 1184;     // partial sums of one launch, 8 per SM; fixed, so that the
+                                     // order of the sum is the same whatever else runs
+
+template <int N>
+struct Table {
+  void* g[N];
+  long long n[N];
+  unsigned first[N + 1];  // first chunk of each tensor; [count] is their number
+  uint8_t dtype[N];       // fm_dtype
+  int count;
+};
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// Blocks walk contiguous ranges of the chunks of all tensors.
+template <typename Tab, typename Body>
+__device__ __forceinline__ void walk(const Tab& tab, Body body) {
+  __shared__ int s_at;
+  const unsigned total = tab.first[tab.count];
+  const unsigned lo = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x);
+  const unsigned hi = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
+  for (int i = threadIdx.x; i < tab.count; i += kThreads)
+    if (tab.first[i] <= lo && lo < tab.first[i + 1]) s_at = i;
+  __syncthreads();
+  int at = s_at;
+  for (unsigned c = lo; c < hi; ++c) {
+    while (tab.first[at + 1] <= c) ++at;
+    const long long base = (long long)(c - tab.first[at]) * kChunk;
+    const long long n = tab.n[at];
+    const int len = (int)(n - base < kChunk ? n - base : kChunk);
+    switch (tab.dtype[at]) {
+      case FM_BF16: body(static_cast<__nv_bfloat16*>(tab.g[at]) + base, len); break;
+      case FM_F16: body(static_cast<__half*>(tab.g[at]) + base, len); break;
+      default: body(static_cast<float*>(tab.g[at]) + base, len); break;
+    }
+  }
+}
+
+// Sum of squares of a chunk: 32 to 36 squares per thread in fp32.
+template <typename T>
+__device__ __forceinline__ float chunk_sumsq(const T* g, int len) {
+  constexpr int V = 16 / sizeof(T);
+  float s = 0.f;
+  if (len == kChunk && (reinterpret_cast<uintptr_t>(g) & 15u) == 0) {
+    constexpr int L = kChunk / (V * kThreads);
+    uint4 raw[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(g) + i * kThreads + threadIdx.x);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float f = to_f<T>(e[j]);
+        s = fmaf(f, f, s);
+      }
+    }
+    return s;
+  }
+#pragma unroll 8
+  for (int i = threadIdx.x; i < len; i += kThreads) {
+    const float f = to_f<T>(g[i]);
+    s = fmaf(f, f, s);
+  }
+  return s;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_constant__ Table<N> tab, double* partials) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  double s = 0.0;
+  walk(tab, [&](auto* g, int len) { s += (double)chunk_sumsq(g, len); });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  __shared__ double red[kThreads / 32];
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = red[0];
+    for (int i = 1; i < kThreads / 32; ++i) s += red[i];
+    partials[blockIdx.x] = s;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+grad_norm_result_kernel(const double* partials, int count, double max_norm, float* result) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += kThreads) s += partials[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  __shared__ double red[kThreads / 32];
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = red[0];
+    for (int i = 1; i < kThreads / 32; ++i) s += red[i];
+    const float norm = (float)sqrt(s);
+    const float ratio = (float)max_norm / (norm + 1e-6f);
+    result[0] = norm;
+    result[1] = fabsf(norm) <= 3.402823466e38f ? fminf(ratio, 1.f) : __int_as_float(0x7fc00000);
+  }
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) scale_multi_kernel(const __grid_constant__ Table<N> tab, const float* factor) {
+  const float f = *factor;
+  if (f == 1.f) return;
+  walk(tab, [&](auto* g, int len) {
+    using T = std::remove_pointer_t<decltype(g)>;
+    constexpr int V = 16 / sizeof(T);
+    if (len == kChunk && (reinterpret_cast<uintptr_t>(g) & 15u) == 0) {
+#pragma unroll
+      for (int i = 0; i < kChunk / (V * kThreads); ++i) {
+        uint4* at = reinterpret_cast<uint4*>(g) + i * kThreads + threadIdx.x;
+        uint4 raw = *at;
+        T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = from_f<T>(to_f<T>(e[j]) * f);
+        *at = raw;
+      }
+      return;
+    }
+#pragma unroll 8
+    for (int i = threadIdx.x; i < len; i += kThreads) g[i] = from_f<T>(to_f<T>(g[i]) * f);
+  });
+}
+
+int check_tensors(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count) {
+  if (count < 0) return fail(FM_ERR_INVALID, "negative tensor count");
+  if (count > 0 && (!grads || !numels || !dtypes)) return fail(FM_ERR_INVALID, "null table");
+  for (int i = 0; i < count; ++i) {
+    if (numels[i] < 0 || numels[i] > (int64_t)1 << 38) return fail(FM_ERR_INVALID, "bad element count at %d", i);
+    if (dtypes[i] < FM_BF16 || dtypes[i] > FM_F32) return fail(FM_ERR_UNSUPPORTED, "unknown dtype %d", dtypes[i]);
+    if (numels[i] == 0) continue;
+    if (!grads[i] || reinterpret_cast<uintptr_t>(grads[i]) % dtype_bytes(dtypes[i]) != 0)
+      return fail(FM_ERR_INVALID, "null or misaligned tensor pointer at %d", i);
+  }
+  return FM_OK;
+}
+
+// Fills tables and hands each to `go(table)`.
+template <int N, typename Go>
+int for_tables(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, Go go) {
+  Table<N> tab;
+  tab.count = 0;
+  tab.first[0] = 0;
+  for (int i = 0; i < count; ++i) {
+    if (numels[i] == 0) continue;
+    const long long chunks = (numels[i] + kChunk - 1) / kChunk;
+    if (tab.count == N || tab.first[tab.count] + chunks > 0x7fffffffLL) {
+      const int rc = go(tab);
+      if (rc != FM_OK) return rc;
+      tab.count = 0;
+    }
+    tab.g[tab.count] = const_cast<void*>(grads[i]);
+    tab.n[tab.count] = numels[i];
+    tab.dtype[tab.count] = (uint8_t)dtypes[i];
+    tab.first[tab.count + 1] = tab.first[tab.count] + (unsigned)chunks;
+    ++tab.count;
+  }
+  return tab.count > 0 ? go(tab) : FM_OK;
+}
+
+// A launch ends when its table is full or the next tensor's chunks (at most 2^25) would overflow the
+// 31 bits of the chunk count, so it holds 63 tensors at least.
+int most_launches(int count) { return count / 63 + 1; }
+
+}  // namespace
+}  // namespace fm
+
+extern "C" size_t fm_grad_norm_workspace_bytes(int count) {
+  if (count < 0) return 0;
+  return (size_t)fm::kMaxBlocks * fm::most_launches(count) * sizeof(double);
+}
+
+extern "C" int fm_grad_norm(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count,
+                            double max_norm, float* result, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  using namespace fm;
+  clear_error();
+  int rc = check_tensors(grads, numels, dtypes, count);
+  if (rc != FM_OK) return rc;
+  if (!result || (reinterpret_cast<uintptr_t>(result) & 3u) != 0) return fail(FM_ERR_INVALID, "null or misaligned result");
+  if (!(max_norm >= 0.0)) return fail(FM_ERR_INVALID, "max_norm must not be negative");
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0)
+    return fail(FM_ERR_INVALID, "null or misaligned workspace");
+  if (workspace_bytes < fm_grad_norm_workspace_bytes(count)) return fail(FM_ERR_WORKSPACE, "workspace too small");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  double* partials = static_cast<double*>(workspace);
+  int used = 0;
+  auto go = [&](const auto& tab) -> int {
+    const unsigned total = tab.first[tab.count];
+    const unsigned blocks = total < (unsigned)kMaxBlocks ? total : (unsigned)kMaxBlocks;
+    grad_norm_kernel<<<blocks, kThreads, 0, st>>>(tab, partials + used);
+    used += (int)blocks;
+    FM_CUDA_CHECK(cudaGetLastError());
+    return FM_OK;
+  };
+  rc = count <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, go)
+                            : for_tables<kLargeTable>(grads, numels, dtypes, count, go);
+  if (rc != FM_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = used > 0 && options().pdl != 0 ? 1 : 0;
+  FM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, grad_norm_result_kernel, (const double*)partials, used, max_norm, result));
+  return FM_OK;
+}
+
+extern "C" int fm_scale_multi(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count,
+                              const float* factor, void* stream) {
+  using namespace fm;
+  clear_error();
+  int rc = check_tensors(grads, numels, dtypes, count);
+  if (rc != FM_OK) return rc;
+  if (!factor || (reinterpret_cast<uintptr_t>(factor) & 3u) != 0) return fail(FM_ERR_INVALID, "null or misaligned factor");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](const auto& tab) -> int {
+    const unsigned total = tab.first[tab.count];
+    const unsigned most = (unsigned)sm_count() * 8;
+    scale_multi_kernel<<<total < most ? total : most, kThreads, 0, st>>>(tab, factor);
+    FM_CUDA_CHECK(cudaGetLastError());
+    return FM_OK;
+  };
+  return count <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, go)
+                              : for_tables<kLargeTable>(grads, numels, dtypes, count, go);
+}

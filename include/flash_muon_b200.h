@@ -259,6 +259,84 @@ int fm_muon_step(const fm_muon_group* groups, int ngroups, void* const* workspac
                  size_t workspace_bytes, void* stream);
 
 /*
+ * One parameter group of an AdamW step, for what Muon does not take (embeddings, heads, norms,
+ * biases).  All arrays are HOST arrays of `count` entries.  Tensor i has numels[i] contiguous
+ * elements: params[i] (p_dtype), grads[i] (g_dtype: p_dtype or FM_F32 for 16-bit parameters, any for
+ * FM_F32), masters[i] (masters null: none; float copies that carry the bits a 16-bit parameter
+ * loses).  steps[i] is a float on the device, the tensor's step count: the call adds one to it and
+ * uses the result.
+ * state_bits 32: exp_avg[i], exp_avg_sq[i] are numels[i] floats.
+ * state_bits 8: they are 16-byte aligned codes, one byte per element, padded to a multiple of 32
+ * bytes; exp_avg_scale[i] and exp_avg_sq_scale[i] hold one byte per 32 elements.  All zero bytes are
+ * zero moments.  First moment: sign | e4m3 times 2^(scale - 134); second: unsigned e5m3 times
+ * 2^(scale - 127) in units where code 248 is 1.  Codes are rounded up or down at random with the
+ * chance of the distance; the random numbers are a function of seeds[i], the step count and the
+ * element's index, so equal calls give equal bits.  A value that is not finite becomes "not a
+ * number" (first moment, code 127) or infinity (second, code 255) and leaves its neighbours alone.
+ */
+typedef struct {
+  void* const* params;
+  const void* const* grads;
+  void* const* masters;
+  void* const* exp_avg;
+  void* const* exp_avg_sq;
+  void* const* exp_avg_scale;
+  void* const* exp_avg_sq_scale;
+  float* const* steps;
+  const int64_t* numels;
+  const uint32_t* seeds;
+  int32_t count;
+  int32_t p_dtype;
+  int32_t g_dtype;
+  int32_t state_bits;     /* 32 or 8 */
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+  const float* lr_device; /* null, or a device float that stands in for lr (schedules inside a graph) */
+} fm_adamw_group;
+
+/*
+ * One AdamW step of every tensor of every group, in place:
+ *   g' = s g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+ *   w = w (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in fp32, each stored value rounded once; 8-bit moments enter w before they are rounded.
+ * grad_scale (may be null: 1) is a device float, e.g. the factor fm_grad_norm leaves; if it is not
+ * finite the step is not taken: nothing is written, the counts included.
+ * Tensors of one kind (types, masters, state bits) share launches, up to 360 tensors and 8 groups
+ * each.  The call needs no workspace and can be captured in a CUDA graph.  Calls on different
+ * streams must not share a tensor.  Memory that is written and overlaps other memory of the call is
+ * refused.
+ */
+int fm_adamw_step(const fm_adamw_group* groups, int ngroups, const float* grad_scale, void* stream);
+
+/* The values (out_dtype) that n 8-bit state codes stand for; moment 1 = exp_avg, 2 = exp_avg_sq.
+ * FM_BF16 and FM_F32 hold them exactly (four significant bits). */
+int fm_adamw8_values(const void* codes, const void* scales, int64_t n, int moment, void* out, int out_dtype,
+                     void* stream);
+/* Codes and scales of n values, rounded to nearest; writes the padding up to a multiple of 32 too. */
+int fm_adamw8_encode(const void* values, int v_dtype, int64_t n, int moment, void* codes, void* scales,
+                     void* stream);
+
+/*
+ * Euclidean norm over all elements of `count` gradients (HOST arrays; dtypes[i] per tensor) and the
+ * factor that clips it: result[0] = norm, result[1] = min(1, max_norm / (norm + 1e-6)), two device
+ * floats.  A norm that is not finite (squares are formed in fp32: from 1.8e19 on) gives the factor
+ * NaN, with which fm_adamw_step takes no step.  max_norm may be infinite: factor 1.
+ * Partial sums are added in 64 bits in a fixed order: equal calls give equal bits.
+ * workspace: fm_grad_norm_workspace_bytes(count) bytes of 8-byte aligned device scratch.
+ */
+size_t fm_grad_norm_workspace_bytes(int count);
+int fm_grad_norm(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count,
+                 double max_norm, float* result, void* workspace, size_t workspace_bytes, void* stream);
+
+/* grads[i] <- round(grads[i] * *factor) for `count` tensors, in place; `factor` is a device float.  With a
+ * factor of exactly 1 nothing is read or written. */
+int fm_scale_multi(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count,
+                   const float* factor, void* stream);
+
+/*
  * Peer-memory plumbing of the copy-engine all-gather that stands in for
  * dist.all_gather_into_tensor (flash_muon/muon.py:108) inside one NVLink-connected box.  Each rank
  * copies its finished slot into every peer's gather buffer with DMA engines and orders the
