@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "common.cuh"
@@ -21,8 +22,9 @@
 namespace fm {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kChunk = 4096;       // elements a block takes at a time; a tensor's last chunk is short
+constexpr int kThreads = 128;
+constexpr int kTile32 = 1024;      // elements of a block, 8 per thread, with 32-bit states
+constexpr int kTile8 = 2048;       // 16 per thread, with 8-bit states: two threads share a block of 32
 constexpr int kMaxHyper = 8;       // parameter groups of one launch
 constexpr int kSmallTable = 40;    // tensors of one launch: the table travels as a kernel argument,
 constexpr int kLargeTable = 360;   // small (4 KB) where it suffices, else up to the limit of 32764 bytes
@@ -43,14 +45,14 @@ struct Entry {
   uint16_t vec;      // every pointer allows 16-byte accesses
 };
 struct Hyper {
-  double lr, beta1, beta2;
-  const float* lr_dev;  // overrides lr where set
-  float eps, wd;
+  double lr, beta1, beta2, wd;
+  const float* lr_dev;            // overrides lr where set
+  float b1, omb1, b2, omb2, eps;  // betas, 1 - betas
 };
 template <int N>
 struct Table {
   Entry e[N];
-  unsigned first[N + 1];  // first chunk of each tensor; [count] is their number
+  unsigned first[N + 1];  // first tile of each tensor; [count] is their number
   Hyper h[kMaxHyper];
   const float* scale;
   int count;
@@ -61,8 +63,9 @@ struct CountTable {
   int count;
 };
 
+// What depends on a tensor's step count.
 struct Coef {
-  float b1, omb1, b2, omb2, eps, decay, size, root;
+  float size, root, decay;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
   uint32_t key;
 };
 
@@ -103,221 +106,395 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466
 // A step whose factor is not finite (the norm it came from was not) is not taken at all.
 __device__ __forceinline__ bool skipped(const float* scale) { return scale != nullptr && !finite(*scale); }
 
-__device__ __forceinline__ Coef coefficients(const Hyper& h, const Entry& e) {
-  const unsigned t = (unsigned)*e.step;
-  const double lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
-  Coef c;
-  c.b1 = (float)h.beta1;
-  c.omb1 = (float)(1.0 - h.beta1);
-  c.b2 = (float)h.beta2;
-  c.omb2 = (float)(1.0 - h.beta2);
-  c.eps = h.eps;
-  c.decay = (float)(1.0 - lr * (double)h.wd);
-  c.size = (float)(lr / (1.0 - power(h.beta1, t)));
-  c.root = (float)(1.0 / sqrt(1.0 - power(h.beta2, t)));
-  c.key = state8::step_key(e.seed, t);
-  return c;
+// Tensor of a tile.  Every thread searches for itself: the table is in constant memory, all lanes
+// read the same word, and no barrier stands before the loads of the tile.
+template <typename Tab>
+__device__ __forceinline__ int find(const Tab& tab, unsigned tile) {
+  int lo = 0, hi = tab.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.first[mid] <= tile) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
-__device__ __forceinline__ void moments(const Coef& c, float g, float& m, float& v) {
-  m = fmaf(c.b1, m, c.omb1 * g);
-  v = fmaf(c.b2, v, c.omb2 * (g * g));
+// The coefficients of the block's tensor, one per warp's first thread, behind the loads of its tile:
+// reading the count and the powers (17 dependent 64-bit products at t = 100000) take less than the
+// loads do.
+__device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, Coef* c) {
+  // the counts are the previous launch's
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if ((threadIdx.x & 31) == 0) {
+    const unsigned t = (unsigned)*reinterpret_cast<const volatile float*>(e.step);
+    const int which = threadIdx.x >> 5;
+    if (which == 0) {
+      const float lr = h.lr_dev ? *h.lr_dev : (float)h.lr;
+      c->size = lr / (float)(1.0 - power(h.beta1, t));
+    } else if (which == 1) {
+      c->root = 1.f / sqrtf((float)(1.0 - power(h.beta2, t)));
+    } else if (which == 2) {
+      c->key = state8::step_key(e.seed, t);
+    } else {
+      c->decay = (float)(1.0 - (h.lr_dev ? (double)*h.lr_dev : h.lr) * h.wd);
+    }
+  }
+  __syncthreads();
 }
 
 // ---------------------------------------------------------------- step counts
 // The counts are advanced by a launch of their own ahead of the step's: every block of the step
-// reads its tensor's count, so none of them may write it.
+// reads its tensor's count, so none of them may write it.  The step's blocks start while it runs
+// and load their tiles: all that those hold was written before this launch began.
 __global__ void __launch_bounds__(kThreads) adamw_count_kernel(const __grid_constant__ CountTable tab) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (skipped(tab.scale)) return;
   for (int i = threadIdx.x; i < tab.count; i += kThreads) *tab.step[i] += 1.f;
 }
 
-// Blocks of a step walk contiguous ranges of the chunks of all tensors.  `body(entry, base, coef)` does
-// one chunk.
-template <typename Tab, typename Body>
-__device__ __forceinline__ void walk(const Tab& tab, Body body) {
-  __shared__ int s_at;
-  __shared__ Coef s_coef;
-  const unsigned total = tab.first[tab.count];
-  const unsigned lo = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x);
-  const unsigned hi = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
-  for (int i = threadIdx.x; i < tab.count; i += kThreads)
-    if (tab.first[i] <= lo && lo < tab.first[i + 1]) s_at = i;
-  // the counts of this step are the previous launch's
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (skipped(tab.scale)) return;
-  const float scale = tab.scale ? *tab.scale : 1.f;
-  __syncthreads();
-  int at = s_at;
-  Coef coef;
-  for (unsigned c = lo; c < hi;) {
-    __syncthreads();
-    if (threadIdx.x == 0) s_coef = coefficients(tab.h[tab.e[at].hyper], tab.e[at]);
-    __syncthreads();
-    coef = s_coef;
-    const unsigned first = tab.first[at], end = min(tab.first[at + 1], hi);
-    for (; c < end; ++c) body(tab.e[at], (long long)(c - first) * kChunk, coef, scale);
-    ++at;
-  }
-}
-
 // ---------------------------------------------------------------- states in fp32
 template <typename P, typename G, bool kMaster, int N>
-__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ Table<N> tab) {
-  walk(tab, [](const Entry& e, long long base, const Coef& c, float scale) {
-    P* const p = static_cast<P*>(e.p);
-    const G* const g = static_cast<const G*>(e.g);
-    float* const m = static_cast<float*>(e.m);
-    float* const v = static_cast<float*>(e.v);
-    auto update = [&](float w, float gr, float& mm, float& vv) {
-      moments(c, gr * scale, mm, vv);
-      return fmaf(w, c.decay, -c.size * (mm / fmaf(sqrtf(vv), c.root, c.eps)));
-    };
-    if (e.vec && base + kChunk <= e.n) {
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> tab) {
+  __shared__ Coef s_coef;
+  const int ti = find(tab, blockIdx.x);
+  const Entry& e = tab.e[ti];
+  const Hyper& h = tab.h[e.hyper];
+  const long long base = (long long)(blockIdx.x - tab.first[ti]) * kTile32;
+  P* const p = static_cast<P*>(e.p) + base;
+  const G* const g = static_cast<const G*>(e.g) + base;
+  float* const w = e.w + base;
+  float* const m = static_cast<float*>(e.m) + base;
+  float* const v = static_cast<float*>(e.v) + base;
+  const bool vec = e.vec && base + kTile32 <= e.n;
+  const int len = (int)(e.n - base < kTile32 ? e.n - base : kTile32);
+  alignas(16) P pv[8];
+  alignas(16) G gv[8];
+  alignas(16) float mv[8], vv[8], wv[8];
+  if (vec) {  // 8 neighbouring elements
+    const int at = threadIdx.x * 8;
+    if (kMaster) load_vec(w + at, wv);
+    else load_vec(p + at, pv);
+    load_vec(g + at, gv);
+    load_vec(m + at, mv);
+    load_vec(v + at, vv);
+  } else {    // 8 elements kThreads apart
 #pragma unroll
-      for (int i = 0; i < kChunk / (8 * kThreads); ++i) {
-        const long long at = base + (i * kThreads + threadIdx.x) * 8;
-        alignas(16) P pv[8];
-        alignas(16) G gv[8];
-        alignas(16) float mv[8], vv[8], wv[8];
-        if (kMaster) load_vec(e.w + at, wv);
-        else load_vec(p + at, pv);
-        load_vec(g + at, gv);
-        load_vec(m + at, mv);
-        load_vec(v + at, vv);
+    for (int j = 0; j < 8; ++j) {
+      const int at = j * kThreads + threadIdx.x;
+      const bool here = at < len;
+      if (kMaster) wv[j] = here ? w[at] : 0.f;
+      else pv[j] = here ? p[at] : from_f<P>(0.f);
+      gv[j] = here ? g[at] : from_f<G>(0.f);
+      mv[j] = here ? m[at] : 0.f;
+      vv[j] = here ? v[at] : 0.f;
+    }
+  }
+  const float scale = tab.scale ? *tab.scale : 1.f;
+  coefficients(h, e, &s_coef);
+  if (!finite(scale)) return;
+  const Coef c = s_coef;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float w = update(kMaster ? wv[j] : to_f<P>(pv[j]), to_f<G>(gv[j]), mv[j], vv[j]);
-          if (kMaster) wv[j] = w;
-          pv[j] = from_f<P>(w);
-        }
-        store_vec(p + at, pv);
-        if (kMaster) store_vec(e.w + at, wv);
-        store_vec(m + at, mv);
-        store_vec(v + at, vv);
+  for (int j = 0; j < 8; ++j) {
+    const float gr = to_f<G>(gv[j]) * scale;
+    mv[j] = fmaf(h.b1, mv[j], h.omb1 * gr);
+    vv[j] = fmaf(h.b2, vv[j], h.omb2 * (gr * gr));
+    wv[j] = fmaf(kMaster ? wv[j] : to_f<P>(pv[j]), c.decay, -c.size * (mv[j] / fmaf(sqrtf(vv[j]), c.root, h.eps)));
+    pv[j] = from_f<P>(wv[j]);
+  }
+  if (vec) {
+    const int at = threadIdx.x * 8;
+    store_vec(p + at, pv);
+    if (kMaster) store_vec(w + at, wv);
+    store_vec(m + at, mv);
+    store_vec(v + at, vv);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = j * kThreads + threadIdx.x;
+      if (at < len) {
+        p[at] = pv[j];
+        if (kMaster) w[at] = wv[j];
+        m[at] = mv[j];
+        v[at] = vv[j];
       }
-      return;
     }
-    const long long end = min(base + kChunk, e.n);
-#pragma unroll 4
-    for (long long at = base + threadIdx.x; at < end; at += kThreads) {
-      float mm = m[at], vv = v[at];
-      const float w = update(kMaster ? e.w[at] : to_f<P>(p[at]), to_f<G>(g[at]), mm, vv);
-      p[at] = from_f<P>(w);
-      if (kMaster) e.w[at] = w;
-      m[at] = mm;
-      v[at] = vv;
-    }
-  });
+  }
 }
 
 // ---------------------------------------------------------------- states in 8 bits
-// A thread takes 16 consecutive elements, two neighbouring lanes a block of 32.
-__device__ __forceinline__ uint32_t finite_max(const float (&x)[16]) {
-  uint32_t mx = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) mx = max(mx, __float_as_uint(x[j]) & 0x7fffffffu);
-  if (mx >= 0x7f800000u) {  // an element that is not finite does not set the block's exponent
-    mx = 0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t u = __float_as_uint(x[j]) & 0x7fffffffu;
-      if (u < 0x7f800000u) mx = max(mx, u);
-    }
-  }
-  return max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+// A thread takes 16 consecutive elements, two neighbouring lanes a block of 32.  The bytes of a
+// step are few enough (10 per bf16 element) that instructions bound it, so arithmetic goes by pairs
+// (fp32x2) and the codes are handled as floats where the hardware converts them:
+//   decode m: e4m3 pairs to f16 pairs, exact; v: the code shifted to bit 7 IS an f16 number;
+//   encode: scaled by the block's power of two (state8.cuh) the code is the bits above bit 20, the
+//   random number is added below and cut off.
+// Two cases that hardly ever occur leave this path: a block whose largest magnitude is not finite or
+// beyond what one fp32 factor scales, and a positive v whose code came out 0.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
 }
+__device__ __forceinline__ void unpack2(f32x2 x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float x) { return pack2(x, x); }
+// within 1 ulp of the root and the reciprocal, subnormal arguments taken as zero
+__device__ __forceinline__ float root_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// the larger one; not a number if one of them is not
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 halves_to_floats(uint32_t h2) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+  return pack2(f.x, f.y);
+}
+// 8 * kThreads + tid ... : a word of padding per 16, so that a thread's 16 elements and a warp's
+// neighbouring ones are both free of bank conflicts
+__device__ __forceinline__ int padded(int i) { return i + (i >> 4); }
+
+// From these block maxima on (bit patterns) one fp32 factor, subnormals among them, no longer scales
+// a block to its codes: 2^(14 - b) and 2^(29 - b) need b <= 163 and b <= 178.
+constexpr uint32_t kFastMaxM = 164u << 23, kFastMaxV = 179u << 23;
 
 template <typename P, typename G, bool kMaster, int N>
-__global__ void __launch_bounds__(kThreads, 2) adamw8_kernel(const __grid_constant__ Table<N> tab) {
-  walk(tab, [](const Entry& e, long long base, const Coef& c, float scale) {
-    P* const p = static_cast<P*>(e.p);
-    const G* const g = static_cast<const G*>(e.g);
-    const long long at = base + threadIdx.x * 16;
-    const long long left = e.n - at;                       // elements of this thread's 16 that exist
-    const bool in = at < (e.n + 31) / 32 * 32;             // its block does
-    const bool full = left >= 16;
-    uint8_t* const mc = static_cast<uint8_t*>(e.m) + at;
-    uint8_t* const vc = static_cast<uint8_t*>(e.v) + at;
-    alignas(16) uint8_t mq[16], vq[16];
-    int mb = 127, vb = 127;
-    alignas(16) float w[16];
-    alignas(16) P pv[16];
-    alignas(16) G gv[16];
-    if (in) {
-      *reinterpret_cast<uint4*>(mq) = *reinterpret_cast<const uint4*>(mc);
-      *reinterpret_cast<uint4*>(vq) = *reinterpret_cast<const uint4*>(vc);
-      mb = e.ms[at >> 5];
-      vb = e.vs[at >> 5];
-    } else {
-      *reinterpret_cast<uint4*>(mq) = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(vq) = make_uint4(0, 0, 0, 0);
-    }
-    if (full && e.vec) {
-      load_vec(g + at, gv);
-      if (kMaster) load_vec(e.w + at, w);
-      else load_vec(p + at, pv);
-    } else {
+__global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant__ Table<N> tab) {
+  __shared__ Coef s_coef;
+  __shared__ float s_w[kTile8 / 16 * 17], s_g[kTile8 / 16 * 17];
+  const int ti = find(tab, blockIdx.x);
+  const Entry& e = tab.e[ti];
+  const Hyper& h = tab.h[e.hyper];
+  const long long base = (long long)(blockIdx.x - tab.first[ti]) * kTile8;
+  const long long at = base + threadIdx.x * 16;
+  P* const p = static_cast<P*>(e.p) + base;
+  const G* const g = static_cast<const G*>(e.g) + base;
+  float* const wp = e.w + base;
+  const bool vec = e.vec && base + kTile8 <= e.n;
+  const int len = (int)(e.n - base < kTile8 ? e.n - base : kTile8);
+  const bool in = at < (e.n + 31) / 32 * 32;  // the thread's block of 32 exists
+  uint4 mq = make_uint4(0, 0, 0, 0), vq = mq;
+  int mb = 127, vb = 127;
+  if (in) {
+    mq = *reinterpret_cast<const uint4*>(static_cast<uint8_t*>(e.m) + at);
+    vq = *reinterpret_cast<const uint4*>(static_cast<uint8_t*>(e.v) + at);
+    mb = e.ms[at >> 5];
+    vb = e.vs[at >> 5];
+  }
+  alignas(16) P pv[16];
+  alignas(16) G gv[16];
+  alignas(16) float wv[16];
+  if (vec) {
+    load_vec(g + threadIdx.x * 16, gv);
+    if (kMaster) load_vec(wp + threadIdx.x * 16, wv);
+    else load_vec(p + threadIdx.x * 16, pv);
+  } else {  // through shared memory: neighbouring threads read neighbouring elements
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const bool here = j < left;
-        gv[j] = here ? g[at + j] : from_f<G>(0.f);
-        if (kMaster) w[j] = here ? e.w[at + j] : 0.f;
-        else pv[j] = here ? p[at + j] : from_f<P>(0.f);
+    for (int j = 0; j < 16; ++j) {
+      const int i = j * kThreads + threadIdx.x;
+      s_g[padded(i)] = i < len ? to_f<G>(g[i]) : 0.f;
+      s_w[padded(i)] = i < len ? (kMaster ? wp[i] : to_f<P>(p[i])) : 0.f;
+    }
+    // bytes behind the last element count as zeros
+    const int left = len - (int)threadIdx.x * 16;
+    uint32_t* mw = reinterpret_cast<uint32_t*>(&mq);
+    uint32_t* vw = reinterpret_cast<uint32_t*>(&vq);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int bytes = left - 4 * k;
+      const uint32_t keep = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
+      mw[k] &= keep;
+      vw[k] &= keep;
+    }
+  }
+  const float scale = tab.scale ? *tab.scale : 1.f;
+  coefficients(h, e, &s_coef);  // its barrier also ends the staging above
+  if (!finite(scale)) return;
+  const Coef c = s_coef;
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      gv[j] = from_f<G>(s_g[padded(threadIdx.x * 16 + j)]);
+      const float x = s_w[padded(threadIdx.x * 16 + j)];
+      if (kMaster) wv[j] = x;
+      else pv[j] = from_f<P>(x);
+    }
+  }
+
+  float m[16], v[16];
+  // 2^(b - 134) and 2^(b - 141) times the codes read as e4m3 and f16; a scale byte of 0 (fresh
+  // states) has only zero codes
+  const f32x2 mf = both(state8::pow2(mb > 17 ? mb - 7 : 10)), vf = both(state8::pow2(vb > 32 ? vb - 14 : 18));
+  const f32x2 b1 = both(h.b1), o1 = both(h.omb1), b2 = both(h.b2), o2 = both(h.omb2), sc = both(scale);
+  const f32x2 root = both(c.root), eps = both(h.eps), decay = both(c.decay), size = both(-c.size);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t mw = reinterpret_cast<uint32_t*>(&mq)[k], vw = reinterpret_cast<uint32_t*>(&vq)[k];
+    // a code with five exponent bits set: infinity among them
+    const bool top = (((vw & 0x78787878u) + 0x08080808u) & vw & 0x80808080u) != 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int j = 4 * k + 2 * q;
+      uint32_t mh;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(mh) : "h"((unsigned short)(mw >> (16 * q))));
+      f32x2 m2 = mul2(halves_to_floats(mh), mf);
+      f32x2 v2 = mul2(halves_to_floats(__byte_perm(vw, 0, q ? 0x4342 : 0x4140) << 7), vf);
+      if (top) {
+        const uint32_t lo = (vw >> (16 * q)) & 0xffu, hi = (vw >> (16 * q + 8)) & 0xffu;
+        v2 = pack2(state8::decode_v((uint8_t)lo, vb), state8::decode_v((uint8_t)hi, vb));
       }
-    }
-    float m[16], v[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const bool here = full || j < left;  // bytes behind the last element count as zeros
-      m[j] = here ? state8::decode_m(mq[j], mb) : 0.f;
-      v[j] = here ? state8::decode_v(vq[j], vb) : 0.f;
-      moments(c, to_f<G>(gv[j]) * scale, m[j], v[j]);
-      if (!kMaster) w[j] = to_f<P>(pv[j]);
+      const f32x2 g2 = mul2(pack2(to_f<G>(gv[j]), to_f<G>(gv[j + 1])), sc);
+      m2 = fma2(b1, m2, mul2(o1, g2));
+      v2 = fma2(b2, v2, mul2(o2, mul2(g2, g2)));
+      unpack2(m2, m[j], m[j + 1]);
+      unpack2(v2, v[j], v[j + 1]);
       // the update takes the moments before they are rounded to 8 bits
-      w[j] = fmaf(w[j], c.decay, -c.size * (m[j] / fmaf(sqrtf(v[j]), c.root, c.eps)));
-      pv[j] = from_f<P>(w[j]);
+      f32x2 d2 = fma2(pack2(root_approx(v[j]), root_approx(v[j + 1])), root, eps);
+      float d0, d1;
+      unpack2(d2, d0, d1);
+      d2 = mul2(m2, pack2(rcp_approx(d0), rcp_approx(d1)));
+      const f32x2 w2 = kMaster ? pack2(wv[j], wv[j + 1]) : pack2(to_f<P>(pv[j]), to_f<P>(pv[j + 1]));
+      unpack2(fma2(w2, decay, mul2(size, d2)), wv[j], wv[j + 1]);
+      pv[j] = from_f<P>(wv[j]);
+      pv[j + 1] = from_f<P>(wv[j + 1]);
     }
-    mb = state8::block_exp(finite_max(m), state8::kMinExpM);
-    vb = state8::block_exp(finite_max(v), state8::kMinExpV);
-    const uint32_t key = state8::index_key(c.key, (uint32_t)(at >> 32));
+  }
+  float mx = fabsf(m[0]), vx = v[0];
+#pragma unroll
+  for (int j = 1; j < 16; ++j) {
+    mx = max_nan(mx, fabsf(m[j]));
+    vx = max_nan(vx, v[j]);
+  }
+  uint32_t mt = __float_as_uint(mx) & 0x7fffffffu, vt = __float_as_uint(vx) & 0x7fffffffu;
+  mt = max(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+  vt = max(vt, __shfl_xor_sync(0xffffffffu, vt, 1));
+  const uint32_t key = state8::index_key(c.key, (uint32_t)(at >> 32)) ^ (uint32_t)at;  // at + j = at ^ j
+  if (mt < kFastMaxM && vt < kFastMaxV) {
+    mb = state8::block_exp(mt, state8::kMinExpM);
+    vb = state8::block_exp(vt, state8::kMinExpV);
+    // 2^(14 - b) and 2^(29 - b), subnormal from b = 141 and 156 on
+    const f32x2 me = both(mb <= 140 ? state8::pow2(141 - mb) : __uint_as_float(0x00800000u >> (mb - 140)));
+    const f32x2 ve = both(vb <= 155 ? state8::pow2(156 - vb) : __uint_as_float(0x00800000u >> (vb - 155)));
+    const f32x2 up = both(state8::pow2(127 + 120));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t x[4];
+      unsigned short half[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int j = 4 * k + 2 * q;
+        const uint32_t h0 = state8::mix(key ^ (uint32_t)j), h1 = state8::mix(key ^ (uint32_t)(j + 1));
+        float y0, y1;
+        unpack2(mul2(pack2(m[j], m[j + 1]), me), y0, y1);
+        y0 = __uint_as_float((__float_as_uint(y0) + state8::random_m(h0)) & 0xfff00000u);
+        y1 = __uint_as_float((__float_as_uint(y1) + state8::random_m(h1)) & 0xfff00000u);
+        unpack2(mul2(pack2(y0, y1), up), y0, y1);
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(half[q]) : "f"(y1), "f"(y0));
+        unpack2(mul2(pack2(v[j], v[j + 1]), ve), y0, y1);
+        x[2 * q] = (__float_as_uint(y0) + state8::random_v(h0)) << 4;
+        x[2 * q + 1] = (__float_as_uint(y1) + state8::random_v(h1)) << 4;
+      }
+      reinterpret_cast<uint32_t*>(&mq)[k] = (uint32_t)half[0] | (uint32_t)half[1] << 16;
+      uint32_t vw = __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410);
+      if (((vw - 0x01010101u) & ~vw & 0x80808080u) != 0) {  // some code is 0
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v[4 * k + j] > 0.f && (vw >> (8 * j) & 0xffu) == 0) vw |= 1u << (8 * j);
+      }
+      reinterpret_cast<uint32_t*>(&vq)[k] = vw;
+    }
+  } else {
+    // an element that is not finite does not set the block's exponent
+    mt = vt = 0;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const uint32_t h = state8::random_bits(key, (uint32_t)at + j);
-      mq[j] = state8::encode_m(m[j], mb, state8::random_m(h));
-      vq[j] = state8::encode_v(v[j], vb, state8::random_v(h));
+      const uint32_t a = __float_as_uint(m[j]) & 0x7fffffffu, b = __float_as_uint(v[j]) & 0x7fffffffu;
+      if (a < 0x7f800000u) mt = max(mt, a);
+      if (b < 0x7f800000u) vt = max(vt, b);
     }
-    if (!in) return;
-    *reinterpret_cast<uint4*>(mc) = *reinterpret_cast<uint4*>(mq);
-    *reinterpret_cast<uint4*>(vc) = *reinterpret_cast<uint4*>(vq);
+    const unsigned pair = 3u << (threadIdx.x & 30);
+    mt = max(mt, __shfl_xor_sync(pair, mt, 1));
+    vt = max(vt, __shfl_xor_sync(pair, vt, 1));
+    mb = state8::block_exp(mt, state8::kMinExpM);
+    vb = state8::block_exp(vt, state8::kMinExpV);
+    alignas(16) uint8_t mc[16], vc[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t r = state8::mix(key ^ (uint32_t)j);
+      mc[j] = state8::encode_m(m[j], mb, state8::random_m(r));
+      vc[j] = state8::encode_v(v[j], vb, state8::random_v(r));
+    }
+    mq = *reinterpret_cast<uint4*>(mc);
+    vq = *reinterpret_cast<uint4*>(vc);
+  }
+  if (in) {
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(e.m) + at) = mq;
+    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(e.v) + at) = vq;
     if ((threadIdx.x & 1) == 0) {
       e.ms[at >> 5] = (uint8_t)mb;
       e.vs[at >> 5] = (uint8_t)vb;
     }
-    if (full && e.vec) {
-      store_vec(p + at, pv);
-      if (kMaster) store_vec(e.w + at, w);
-    } else {
+  }
+  if (vec) {
+    store_vec(p + threadIdx.x * 16, pv);
+    if (kMaster) store_vec(wp + threadIdx.x * 16, wv);
+  } else {
+    // a thread overwrites only what it alone has read
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (j < left) {
-          p[at + j] = pv[j];
-          if (kMaster) e.w[at + j] = w[j];
-        }
+    for (int j = 0; j < 16; ++j) s_w[padded(threadIdx.x * 16 + j)] = wv[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int i = j * kThreads + threadIdx.x;
+      if (i < len) {
+        const float x = s_w[padded(i)];
+        p[i] = from_f<P>(x);
+        if (kMaster) wp[i] = x;
       }
     }
-  });
+  }
 }
 
 // ---------------------------------------------------------------- 8-bit states to values and back
-template <typename T>
+// 16 codes per thread (`vec`: both addresses allow 16-byte accesses), the rest one by one.
+template <typename T, int kMoment>
 __global__ void __launch_bounds__(kThreads)
-adamw8_values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int moment, T* out) {
-  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
-    const int b = exps[i >> 5];
-    out[i] = from_f<T>(moment == 1 ? state8::decode_m(codes[i], b) : state8::decode_v(codes[i], b));
+adamw8_values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int vec, T* out) {
+  const long long at = ((long long)blockIdx.x * kThreads + threadIdx.x) * 16;
+  if (at >= n) return;
+  const int b = exps[at >> 5];
+  auto value = [&](uint8_t c) { return kMoment == 1 ? state8::decode_m(c, b) : state8::decode_v(c, b); };
+  if (vec && at + 16 <= n) {
+    alignas(16) uint8_t c[16];
+    alignas(16) T x[16];
+    *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(codes + at);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = from_f<T>(value(c[j]));
+    store_vec(out + at, x);
+    return;
   }
+  for (int j = 0; j < 16 && at + j < n; ++j) out[at + j] = from_f<T>(value(codes[at + j]));
 }
 
 // One warp per block of 32, rounding to nearest.
@@ -419,16 +596,8 @@ Kind kind_of(const fm_adamw_group& g) { return {g.p_dtype, g.g_dtype, g.state_bi
 
 template <auto kernel, typename Tab>
 int launch_table(const Tab& tab, bool dependent, cudaStream_t stream) {
-  static int resident = 0;  // blocks per SM of this kernel
-  if (resident == 0) {
-    int per_sm = 0;
-    FM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0));
-    resident = per_sm > 0 ? per_sm : 1;
-  }
-  const long long most = (long long)resident * sm_count();
-  const long long total = tab.first[tab.count];
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(total < most ? total : most));
+  cfg.gridDim = dim3(tab.first[tab.count]);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
@@ -500,9 +669,10 @@ struct Batch {
 
   int add(const fm_adamw_group& g, int gi, int i) {
     const int64_t n = g.numels[i];
-    const int64_t chunks = (n + kChunk - 1) / kChunk;
+    const int tile = g.state_bits == 8 ? kTile8 : kTile32;
+    const int64_t tiles = (n + tile - 1) / tile;
     if (tab.count > 0 && (tab.count == kLargeTable || (last_group != gi && hypers == kMaxHyper) ||
-                          tab.first[tab.count] + chunks > 0x7fffffffLL)) {
+                          tab.first[tab.count] + tiles > 0x7fffffffLL)) {
       const int rc = flush();
       if (rc != FM_OK) return rc;
     }
@@ -510,7 +680,9 @@ struct Batch {
     if (last_group != gi) {
       Hyper& h = tab.h[hypers++];
       h.lr = g.lr; h.beta1 = g.beta1; h.beta2 = g.beta2; h.lr_dev = g.lr_device;
-      h.eps = (float)g.eps; h.wd = (float)g.weight_decay;
+      h.wd = g.weight_decay; h.eps = (float)g.eps;
+      h.b1 = (float)g.beta1; h.omb1 = (float)(1.0 - g.beta1);
+      h.b2 = (float)g.beta2; h.omb2 = (float)(1.0 - g.beta2);
       last_group = gi;
     }
     Entry& e = tab.e[tab.count];
@@ -524,7 +696,7 @@ struct Batch {
     e.seed = g.state_bits == 8 ? g.seeds[i] : 0;
     e.hyper = (uint16_t)(hypers - 1);
     e.vec = aligned(e.p, 16) && aligned(e.g, 16) && aligned(e.w, 16) && aligned(e.m, 16) && aligned(e.v, 16);
-    tab.first[tab.count + 1] = tab.first[tab.count] + (unsigned)chunks;
+    tab.first[tab.count + 1] = tab.first[tab.count] + (unsigned)tiles;
     ++tab.count;
     return FM_OK;
   }
@@ -598,7 +770,7 @@ int simple_grid(long long n) {
 }
 
 int check_moment(const void* a, const void* b, const void* c, int64_t n, int moment) {
-  if (n < 0) return fail(FM_ERR_INVALID, "negative element count");
+  if (n < 0 || n > (int64_t)1 << 38) return fail(FM_ERR_INVALID, "bad element count");
   if (moment != 1 && moment != 2) return fail(FM_ERR_INVALID, "moment must be 1 or 2");
   if (n > 0 && (!a || !b || !c)) return fail(FM_ERR_INVALID, "null pointer");
   return FM_OK;
@@ -629,13 +801,16 @@ extern "C" int fm_adamw8_values(const void* codes, const void* scales, int64_t n
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int grid = simple_grid(n);
-  if (out_dtype == FM_F32)
-    adamw8_values_kernel<float><<<grid, kThreads, 0, st>>>(c, s, n, moment, static_cast<float*>(out));
-  else if (out_dtype == FM_BF16)
-    adamw8_values_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(c, s, n, moment, static_cast<__nv_bfloat16*>(out));
-  else
-    adamw8_values_kernel<__half><<<grid, kThreads, 0, st>>>(c, s, n, moment, static_cast<__half*>(out));
+  const int vec = aligned(codes, 16) && aligned(out, 16);
+  const unsigned grid = (unsigned)((n + kThreads * 16 - 1) / (kThreads * 16));
+  auto go = [&](auto* o) {
+    using T = std::remove_pointer_t<decltype(o)>;
+    if (moment == 1) adamw8_values_kernel<T, 1><<<grid, kThreads, 0, st>>>(c, s, n, vec, o);
+    else adamw8_values_kernel<T, 2><<<grid, kThreads, 0, st>>>(c, s, n, vec, o);
+  };
+  if (out_dtype == FM_F32) go(static_cast<float*>(out));
+  else if (out_dtype == FM_BF16) go(static_cast<__nv_bfloat16*>(out));
+  else go(static_cast<__half*>(out));
   FM_CUDA_CHECK(cudaGetLastError());
   return FM_OK;
 }
