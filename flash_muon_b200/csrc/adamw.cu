@@ -24,7 +24,8 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kTile32 = 1024;      // elements of a block, 8 per thread, with 32-bit states
-constexpr int kTile8 = 2048;       // 16 per thread, with 8-bit states: two threads share a block of 32
+constexpr int kPart8 = 2048;       // 16 per thread with 8-bit states, where two threads share a block of
+constexpr int kMaxParts = 8;       // 32, and a block takes up to 8 such parts
 constexpr int kMaxHyper = 8;       // parameter groups of one launch
 constexpr int kSmallTable = 40;    // tensors of one launch: the table travels as a kernel argument,
 constexpr int kLargeTable = 360;   // small (4 KB) where it suffices, else up to the limit of 32764 bytes
@@ -42,7 +43,7 @@ struct Entry {
   long long n;
   uint32_t seed;
   uint16_t hyper;
-  uint16_t vec;      // every pointer allows 16-byte accesses
+  uint16_t vec;      // every pointer allows the widest accesses made (16-byte codes, 32 bytes else)
 };
 struct Hyper {
   double lr, beta1, beta2, wd;
@@ -56,6 +57,7 @@ struct Table {
   Hyper h[kMaxHyper];
   const float* scale;
   int count;
+  int parts;              // 8-bit states: parts of a tile
 };
 struct CountTable {
   float* step[kCountTable];
@@ -78,18 +80,42 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// N elements from / to a 16-byte aligned address
+// N elements from / to an address aligned to 32 bytes (16 where they are no more): 32 bytes per
+// access where possible.  Two 16-byte stores per thread would each write half of every sector.
 template <typename T, int N>
 __device__ __forceinline__ void load_vec(const T* src, T (&dst)[N]) {
+  constexpr int kBytes = N * sizeof(T);
+  if constexpr (kBytes % 32 == 0) {
+    uint32_t* d = reinterpret_cast<uint32_t*>(dst);
 #pragma unroll
-  for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i)
-    reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    for (int i = 0; i < kBytes / 32; ++i)
+      asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(d[8 * i]), "=r"(d[8 * i + 1]), "=r"(d[8 * i + 2]), "=r"(d[8 * i + 3]), "=r"(d[8 * i + 4]),
+                     "=r"(d[8 * i + 5]), "=r"(d[8 * i + 6]), "=r"(d[8 * i + 7])
+                   : "l"(reinterpret_cast<const char*>(src) + 32 * i)
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i)
+      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+  }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_vec(T* dst, const T (&src)[N]) {
+  constexpr int kBytes = N * sizeof(T);
+  if constexpr (kBytes % 32 == 0) {
+    const uint32_t* d = reinterpret_cast<const uint32_t*>(src);
 #pragma unroll
-  for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i)
-    reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    for (int i = 0; i < kBytes / 32; ++i)
+      asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(d[8 * i]), "r"(d[8 * i + 1]),
+                   "r"(d[8 * i + 2]), "r"(d[8 * i + 3]), "r"(d[8 * i + 4]), "r"(d[8 * i + 5]), "r"(d[8 * i + 6]),
+                   "r"(d[8 * i + 7]), "l"(reinterpret_cast<char*>(dst) + 32 * i)
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i)
+      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+  }
 }
 
 __device__ __forceinline__ double power(double b, unsigned t) {
@@ -122,7 +148,7 @@ __device__ __forceinline__ int find(const Tab& tab, unsigned tile) {
 // The coefficients of the block's tensor, one per warp's first thread, behind the loads of its tile:
 // reading the count and the powers (17 dependent 64-bit products at t = 100000) take less than the
 // loads do.
-__device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, Coef* c) {
+__device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, uint32_t index_hi, Coef* c) {
   // the counts are the previous launch's
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if ((threadIdx.x & 31) == 0) {
@@ -134,7 +160,7 @@ __device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, Coe
     } else if (which == 1) {
       c->root = 1.f / sqrtf((float)(1.0 - power(h.beta2, t)));
     } else if (which == 2) {
-      c->key = state8::step_key(e.seed, t);
+      c->key = state8::index_key(state8::step_key(e.seed, t), index_hi);
     } else {
       c->decay = (float)(1.0 - (h.lr_dev ? (double)*h.lr_dev : h.lr) * h.wd);
     }
@@ -190,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     }
   }
   const float scale = tab.scale ? *tab.scale : 1.f;
-  coefficients(h, e, &s_coef);
+  coefficients(h, e, 0, &s_coef);
   if (!finite(scale)) return;
   const Coef c = s_coef;
 #pragma unroll
@@ -229,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 //   encode: scaled by the block's power of two (state8.cuh) the code is the bits above bit 20, the
 //   random number is added below and cut off.
 // Two cases that hardly ever occur leave this path: a block whose largest magnitude is not finite or
-// beyond what one fp32 factor scales, and a positive v whose code came out 0.
+// beyond what one normal fp32 factor scales, and a positive v whose code came out 0.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack2(float lo, float hi) {
   f32x2 r;
@@ -261,223 +287,306 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// the larger one; not a number if one of them is not
-__device__ __forceinline__ float max_nan(float a, float b) {
+// the largest magnitude; not a number if one of them is not
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ f32x2 halves_to_floats(uint32_t h2) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
   return pack2(f.x, f.y);
 }
-// 8 * kThreads + tid ... : a word of padding per 16, so that a thread's 16 elements and a warp's
-// neighbouring ones are both free of bank conflicts
+// a half that is not a number becomes infinite, others stay
+__device__ __forceinline__ uint32_t at_most_inf(uint32_t h2) {
+  uint32_t r;
+  asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h2), "r"(0x7c007c00u));
+  return r;
+}
+// A word of padding per 16: a thread's 16 elements and a warp's neighbouring ones are both free of
+// bank conflicts.
 __device__ __forceinline__ int padded(int i) { return i + (i >> 4); }
 
-// From these block maxima on (bit patterns) one fp32 factor, subnormals among them, no longer scales
-// a block to its codes: 2^(14 - b) and 2^(29 - b) need b <= 163 and b <= 178.
-constexpr uint32_t kFastMaxM = 164u << 23, kFastMaxV = 179u << 23;
+// Block maxima (bit patterns) below which 2^(14 - b) and 2^(29 - b), which scale a block to its codes,
+// are normal fp32 numbers: moments below 2^14 and 2^29.
+constexpr uint32_t kFastMaxM = 141u << 23, kFastMaxV = 156u << 23;
+
+// 16 bytes from global to shared memory, in the background
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// 2048 elements of type T as 16-byte chunks in shared memory.  A thread's 16 elements are 1, 2 or 4
+// consecutive chunks; their low bits are exchanged with higher ones so that the eight lanes of a
+// shared-memory access find eight different banks.
+template <typename T>
+struct Staged {
+  static constexpr int kPer = sizeof(T);            // chunks per thread
+  static constexpr int kChunks = kThreads * kPer;
+  uint4 c[kChunks];
+  __device__ static int slot(int chunk) { return kPer == 1 ? chunk : chunk ^ ((chunk >> 3) & (kPer - 1)); }
+  __device__ void fetch(const T* src) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int k = i * kThreads + threadIdx.x;
+      copy_async(&c[slot(k)], reinterpret_cast<const uint4*>(src) + k);
+    }
+  }
+  __device__ void read(T (&dst)[16]) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) reinterpret_cast<uint4*>(dst)[i] = c[slot(threadIdx.x * kPer + i)];
+  }
+};
 
 template <typename P, typename G, bool kMaster, int N>
-__global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant__ Table<N> tab) {
+__global__ void __launch_bounds__(kThreads, 6) adamw8_kernel(const __grid_constant__ Table<N> tab) {
+  using W = std::conditional_t<kMaster, float, P>;  // what the weights are read from
+  struct Stage {
+    Staged<uint8_t> m, v;
+    Staged<G> g;
+    Staged<W> w;
+  };
+  struct Plain {  // parts that are not copied in the background
+    float w[kPart8 / 16 * 17], g[kPart8 / 16 * 17];
+  };
+  union Shared {
+    Stage stage[2];
+    Plain plain;
+    __device__ Shared() {}
+  };
+  __shared__ Shared sh;
   __shared__ Coef s_coef;
-  __shared__ float s_w[kTile8 / 16 * 17], s_g[kTile8 / 16 * 17];
+  float* const s_w = sh.plain.w;
+  float* const s_g = sh.plain.g;
   const int ti = find(tab, blockIdx.x);
   const Entry& e = tab.e[ti];
   const Hyper& h = tab.h[e.hyper];
-  const long long base = (long long)(blockIdx.x - tab.first[ti]) * kTile8;
-  const long long at = base + threadIdx.x * 16;
+  const int tile = tab.parts * kPart8;
+  const long long base = (long long)(blockIdx.x - tab.first[ti]) * tile;
+  const unsigned len = (unsigned)(e.n - base < tile ? e.n - base : tile);
+  const unsigned coded = (len + 31) & ~31u;  // codes of this tile
+  const unsigned mine = threadIdx.x * 16;
   P* const p = static_cast<P*>(e.p) + base;
   const G* const g = static_cast<const G*>(e.g) + base;
-  float* const wp = e.w + base;
-  const bool vec = e.vec && base + kTile8 <= e.n;
-  const int len = (int)(e.n - base < kTile8 ? e.n - base : kTile8);
-  const bool in = at < (e.n + 31) / 32 * 32;  // the thread's block of 32 exists
-  uint4 mq = make_uint4(0, 0, 0, 0), vq = mq;
-  int mb = 127, vb = 127;
-  if (in) {
-    mq = *reinterpret_cast<const uint4*>(static_cast<uint8_t*>(e.m) + at);
-    vq = *reinterpret_cast<const uint4*>(static_cast<uint8_t*>(e.v) + at);
-    mb = e.ms[at >> 5];
-    vb = e.vs[at >> 5];
-  }
-  alignas(16) P pv[16];
-  alignas(16) G gv[16];
-  alignas(16) float wv[16];
-  if (vec) {
-    load_vec(g + threadIdx.x * 16, gv);
-    if (kMaster) load_vec(wp + threadIdx.x * 16, wv);
-    else load_vec(p + threadIdx.x * 16, pv);
-  } else {  // through shared memory: neighbouring threads read neighbouring elements
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int i = j * kThreads + threadIdx.x;
-      s_g[padded(i)] = i < len ? to_f<G>(g[i]) : 0.f;
-      s_w[padded(i)] = i < len ? (kMaster ? wp[i] : to_f<P>(p[i])) : 0.f;
-    }
-    // bytes behind the last element count as zeros
-    const int left = len - (int)threadIdx.x * 16;
-    uint32_t* mw = reinterpret_cast<uint32_t*>(&mq);
-    uint32_t* vw = reinterpret_cast<uint32_t*>(&vq);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int bytes = left - 4 * k;
-      const uint32_t keep = bytes >= 4 ? 0xffffffffu : bytes <= 0 ? 0u : (1u << (8 * bytes)) - 1u;
-      mw[k] &= keep;
-      vw[k] &= keep;
-    }
-  }
+  float* const w = e.w + base;
+  uint8_t* const mc = static_cast<uint8_t*>(e.m) + base;
+  uint8_t* const vc = static_cast<uint8_t*>(e.v) + base;
+  uint8_t* const ms = e.ms + (base >> 5);
+  uint8_t* const vs = e.vs + (base >> 5);
   const float scale = tab.scale ? *tab.scale : 1.f;
-  coefficients(h, e, &s_coef);  // its barrier also ends the staging above
-  if (!finite(scale)) return;
-  const Coef c = s_coef;
-  if (!vec) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      gv[j] = from_f<G>(s_g[padded(threadIdx.x * 16 + j)]);
-      const float x = s_w[padded(threadIdx.x * 16 + j)];
-      if (kMaster) wv[j] = x;
-      else pv[j] = from_f<P>(x);
-    }
-  }
 
-  float m[16], v[16];
-  // 2^(b - 134) and 2^(b - 141) times the codes read as e4m3 and f16; a scale byte of 0 (fresh
-  // states) has only zero codes
-  const f32x2 mf = both(state8::pow2(mb > 17 ? mb - 7 : 10)), vf = both(state8::pow2(vb > 32 ? vb - 14 : 18));
-  const f32x2 b1 = both(h.b1), o1 = both(h.omb1), b2 = both(h.b2), o2 = both(h.omb2), sc = both(scale);
-  const f32x2 root = both(c.root), eps = both(h.eps), decay = both(c.decay), size = both(-c.size);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t mw = reinterpret_cast<uint32_t*>(&mq)[k], vw = reinterpret_cast<uint32_t*>(&vq)[k];
-    // a code with five exponent bits set: infinity among them
-    const bool top = (((vw & 0x78787878u) + 0x08080808u) & vw & 0x80808080u) != 0;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int j = 4 * k + 2 * q;
-      uint32_t mh;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(mh) : "h"((unsigned short)(mw >> (16 * q))));
-      f32x2 m2 = mul2(halves_to_floats(mh), mf);
-      f32x2 v2 = mul2(halves_to_floats(__byte_perm(vw, 0, q ? 0x4342 : 0x4140) << 7), vf);
-      if (top) {
-        const uint32_t lo = (vw >> (16 * q)) & 0xffu, hi = (vw >> (16 * q + 8)) & 0xffu;
-        v2 = pack2(state8::decode_v((uint8_t)lo, vb), state8::decode_v((uint8_t)hi, vb));
+  // Whole parts of tensors whose addresses allow it arrive in shared memory two parts ahead.
+  auto fetch = [&](unsigned start, int k) {
+    if (e.vec && start + kPart8 <= len) {
+      Stage& st = sh.stage[k];
+      st.m.fetch(mc + start);
+      st.v.fetch(vc + start);
+      st.g.fetch(g + start);
+      if constexpr (kMaster) st.w.fetch(w + start);
+      else st.w.fetch(p + start);
+    }
+    copy_commit();
+  };
+  fetch(0, 0);
+  fetch(kPart8, 1);
+  int mb_next = 127, vb_next = 127;  // exponent bytes, a part ahead in registers
+  auto fetch_exps = [&](unsigned at) {
+    if (at < coded) {
+      mb_next = ms[at >> 5];
+      vb_next = vs[at >> 5];
+    }
+  };
+  fetch_exps(mine);
+  for (unsigned start = 0, stage = 0; start < len; start += kPart8, stage ^= 1) {
+    const unsigned at = start + mine;
+    const bool vec = e.vec && start + kPart8 <= len;
+    alignas(16) uint8_t mq[16], vq[16];
+    int mb = mb_next, vb = vb_next;
+    alignas(16) W wv[16];
+    alignas(16) G gv[16];
+    fetch_exps(at + kPart8);
+    if (vec) {
+      copy_wait<1>();
+      __syncthreads();
+      const Stage& st = sh.stage[stage];
+      st.m.read(mq);
+      st.v.read(vq);
+      st.g.read(gv);
+      st.w.read(wv);
+      __syncthreads();
+      fetch(start + 2 * kPart8, stage);
+    } else {  // through shared memory: neighbouring threads read neighbouring elements
+      *reinterpret_cast<uint4*>(mq) = *reinterpret_cast<uint4*>(vq) = make_uint4(0, 0, 0, 0);
+      if (at < coded) {
+        *reinterpret_cast<uint4*>(mq) = *reinterpret_cast<const uint4*>(mc + at);
+        *reinterpret_cast<uint4*>(vq) = *reinterpret_cast<const uint4*>(vc + at);
       }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const unsigned i = j * kThreads + threadIdx.x;
+        s_g[padded(i)] = start + i < len ? to_f<G>(g[start + i]) : 0.f;
+        s_w[padded(i)] = start + i < len ? (kMaster ? w[start + i] : to_f<P>(p[start + i])) : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        gv[j] = from_f<G>(s_g[padded(mine + j)]);
+        wv[j] = from_f<W>(s_w[padded(mine + j)]);
+      }
+      // bytes behind the last element count as zeros
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int left = (int)len - (int)at - 4 * k;
+        const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        reinterpret_cast<uint32_t*>(mq)[k] &= keep;
+        reinterpret_cast<uint32_t*>(vq)[k] &= keep;
+      }
+    }
+    if (start == 0) {
+      coefficients(h, e, (uint32_t)(base >> 32), &s_coef);
+      if (!finite(scale)) {
+        copy_wait<0>();
+        return;
+      }
+    }
+    const f32x2 root = both(s_coef.root), decay = both(s_coef.decay), size = both(-s_coef.size);
+    const f32x2 b1 = both(h.b1), o1 = both(h.omb1), b2 = both(h.b2), o2 = both(h.omb2), eps = both(h.eps), sc = both(scale);
+
+    float m[16], v[16];
+    alignas(16) float wn[16];
+    // 2^(b - 134) and 2^(b - 141) times the codes read as e4m3 and f16; a scale byte of 0 (fresh
+    // states) has only zero codes
+    const f32x2 mf = both(state8::pow2(max(mb, state8::kMinExpM) - 7)), vf = both(state8::pow2(max(vb, state8::kMinExpV) - 14));
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const uint32_t mw = reinterpret_cast<uint32_t*>(mq)[j / 4], vw = reinterpret_cast<uint32_t*>(vq)[j / 4];
+      uint32_t mh;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(mh) : "h"((unsigned short)(j & 2 ? mw >> 16 : mw)));
+      f32x2 m2 = mul2(halves_to_floats(mh), mf);
+      // code 255, infinity, comes out of the shift as "not a number"
+      f32x2 v2 = mul2(halves_to_floats(at_most_inf(__byte_perm(vw, 0, j & 2 ? 0x4342 : 0x4140) << 7)), vf);
       const f32x2 g2 = mul2(pack2(to_f<G>(gv[j]), to_f<G>(gv[j + 1])), sc);
       m2 = fma2(b1, m2, mul2(o1, g2));
       v2 = fma2(b2, v2, mul2(o2, mul2(g2, g2)));
       unpack2(m2, m[j], m[j + 1]);
       unpack2(v2, v[j], v[j + 1]);
       // the update takes the moments before they are rounded to 8 bits
-      f32x2 d2 = fma2(pack2(root_approx(v[j]), root_approx(v[j + 1])), root, eps);
       float d0, d1;
-      unpack2(d2, d0, d1);
-      d2 = mul2(m2, pack2(rcp_approx(d0), rcp_approx(d1)));
-      const f32x2 w2 = kMaster ? pack2(wv[j], wv[j + 1]) : pack2(to_f<P>(pv[j]), to_f<P>(pv[j + 1]));
-      unpack2(fma2(w2, decay, mul2(size, d2)), wv[j], wv[j + 1]);
-      pv[j] = from_f<P>(wv[j]);
-      pv[j + 1] = from_f<P>(wv[j + 1]);
+      unpack2(fma2(pack2(root_approx(v[j]), root_approx(v[j + 1])), root, eps), d0, d1);
+      const f32x2 d2 = mul2(m2, pack2(rcp_approx(d0), rcp_approx(d1)));
+      const f32x2 w2 = pack2(to_f<W>(wv[j]), to_f<W>(wv[j + 1]));
+      unpack2(fma2(w2, decay, mul2(size, d2)), wn[j], wn[j + 1]);
     }
-  }
-  float mx = fabsf(m[0]), vx = v[0];
+    if (vec) {
+      alignas(16) P out[16];
 #pragma unroll
-  for (int j = 1; j < 16; ++j) {
-    mx = max_nan(mx, fabsf(m[j]));
-    vx = max_nan(vx, v[j]);
-  }
-  uint32_t mt = __float_as_uint(mx) & 0x7fffffffu, vt = __float_as_uint(vx) & 0x7fffffffu;
-  mt = max(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-  vt = max(vt, __shfl_xor_sync(0xffffffffu, vt, 1));
-  const uint32_t key = state8::index_key(c.key, (uint32_t)(at >> 32)) ^ (uint32_t)at;  // at + j = at ^ j
-  if (mt < kFastMaxM && vt < kFastMaxV) {
-    mb = state8::block_exp(mt, state8::kMinExpM);
-    vb = state8::block_exp(vt, state8::kMinExpV);
-    // 2^(14 - b) and 2^(29 - b), subnormal from b = 141 and 156 on
-    const f32x2 me = both(mb <= 140 ? state8::pow2(141 - mb) : __uint_as_float(0x00800000u >> (mb - 140)));
-    const f32x2 ve = both(vb <= 155 ? state8::pow2(156 - vb) : __uint_as_float(0x00800000u >> (vb - 155)));
-    const f32x2 up = both(state8::pow2(127 + 120));
+      for (int j = 0; j < 16; ++j) out[j] = from_f<P>(wn[j]);
+      store_vec(p + at, out);
+      if (kMaster) store_vec(w + at, wn);
+    } else {  // written from there below; a thread overwrites only what it alone has read
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t x[4];
-      unsigned short half[2];
+      for (int j = 0; j < 16; ++j) s_w[padded(mine + j)] = wn[j];
+    }
+    float mx = max_abs(m[0], m[1], m[2]), vx = max_abs(v[0], v[1], v[2]);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int j = 4 * k + 2 * q;
-        const uint32_t h0 = state8::mix(key ^ (uint32_t)j), h1 = state8::mix(key ^ (uint32_t)(j + 1));
-        float y0, y1;
-        unpack2(mul2(pack2(m[j], m[j + 1]), me), y0, y1);
-        y0 = __uint_as_float((__float_as_uint(y0) + state8::random_m(h0)) & 0xfff00000u);
-        y1 = __uint_as_float((__float_as_uint(y1) + state8::random_m(h1)) & 0xfff00000u);
-        unpack2(mul2(pack2(y0, y1), up), y0, y1);
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(half[q]) : "f"(y1), "f"(y0));
-        unpack2(mul2(pack2(v[j], v[j + 1]), ve), y0, y1);
-        x[2 * q] = (__float_as_uint(y0) + state8::random_v(h0)) << 4;
-        x[2 * q + 1] = (__float_as_uint(y1) + state8::random_v(h1)) << 4;
+    for (int j = 3; j < 15; j += 2) {
+      mx = max_abs(mx, m[j], m[j + 1]);
+      vx = max_abs(vx, v[j], v[j + 1]);
+    }
+    uint32_t mt = __float_as_uint(max_abs(mx, m[15], 0.f)), vt = __float_as_uint(max_abs(vx, v[15], 0.f));
+    mt = max(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+    vt = max(vt, __shfl_xor_sync(0xffffffffu, vt, 1));
+    // mix(key ^ (index + j)) for j < 16: the index's low bits are zero, and the first xor-shift of
+    // the mix does not reach j
+    uint32_t key = s_coef.key ^ ((uint32_t)base + at);
+    key ^= key >> 16;
+    if (mt < kFastMaxM && vt < kFastMaxV) {
+      mb = max((int)(mt >> 23), state8::kMinExpM);
+      vb = max((int)(vt >> 23), state8::kMinExpV);
+      const f32x2 me = both(state8::pow2(141 - mb)), ve = both(state8::pow2(156 - vb)), up = both(state8::pow2(127 + 120));
+      uint32_t zero = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t c[4];
+        unsigned short half[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int j = 4 * k + 2 * q;
+          const uint32_t h0 = state8::mix_folded(key ^ (uint32_t)j), h1 = state8::mix_folded(key ^ (uint32_t)(j + 1));
+          float y0, y1;
+          unpack2(mul2(pack2(m[j], m[j + 1]), me), y0, y1);
+          y0 = __uint_as_float((__float_as_uint(y0) + state8::random_m(h0)) & 0xfff00000u);
+          y1 = __uint_as_float((__float_as_uint(y1) + state8::random_m(h1)) & 0xfff00000u);
+          unpack2(mul2(pack2(y0, y1), up), y0, y1);
+          asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(half[q]) : "f"(y1), "f"(y0));
+          unpack2(mul2(pack2(v[j], v[j + 1]), ve), y0, y1);
+          c[2 * q] = (__float_as_uint(y0) + state8::random_v(h0)) << 4;
+          c[2 * q + 1] = (__float_as_uint(y1) + state8::random_v(h1)) << 4;
+        }
+        reinterpret_cast<uint32_t*>(mq)[k] = (uint32_t)half[0] | (uint32_t)half[1] << 16;
+        const uint32_t vw = __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
+        zero |= (vw - 0x01010101u) & ~vw;
+        reinterpret_cast<uint32_t*>(vq)[k] = vw;
       }
-      reinterpret_cast<uint32_t*>(&mq)[k] = (uint32_t)half[0] | (uint32_t)half[1] << 16;
-      uint32_t vw = __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410);
-      if (((vw - 0x01010101u) & ~vw & 0x80808080u) != 0) {  // some code is 0
+      if (zero & 0x80808080u) {  // some code is 0
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (v[4 * k + j] > 0.f && (vw >> (8 * j) & 0xffu) == 0) vw |= 1u << (8 * j);
+        for (int j = 0; j < 16; ++j) {
+          uint32_t& vw = reinterpret_cast<uint32_t*>(vq)[j / 4];
+          if (v[j] > 0.f && (vw >> (8 * (j & 3)) & 0xffu) == 0) vw |= 1u << (8 * (j & 3));
+        }
       }
-      reinterpret_cast<uint32_t*>(&vq)[k] = vw;
-    }
-  } else {
-    // an element that is not finite does not set the block's exponent
-    mt = vt = 0;
+    } else {
+      mt = vt = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t a = __float_as_uint(m[j]) & 0x7fffffffu, b = __float_as_uint(v[j]) & 0x7fffffffu;
-      if (a < 0x7f800000u) mt = max(mt, a);
-      if (b < 0x7f800000u) vt = max(vt, b);
-    }
-    const unsigned pair = 3u << (threadIdx.x & 30);
-    mt = max(mt, __shfl_xor_sync(pair, mt, 1));
-    vt = max(vt, __shfl_xor_sync(pair, vt, 1));
-    mb = state8::block_exp(mt, state8::kMinExpM);
-    vb = state8::block_exp(vt, state8::kMinExpV);
-    alignas(16) uint8_t mc[16], vc[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t r = state8::mix(key ^ (uint32_t)j);
-      mc[j] = state8::encode_m(m[j], mb, state8::random_m(r));
-      vc[j] = state8::encode_v(v[j], vb, state8::random_v(r));
-    }
-    mq = *reinterpret_cast<uint4*>(mc);
-    vq = *reinterpret_cast<uint4*>(vc);
-  }
-  if (in) {
-    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(e.m) + at) = mq;
-    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(e.v) + at) = vq;
-    if ((threadIdx.x & 1) == 0) {
-      e.ms[at >> 5] = (uint8_t)mb;
-      e.vs[at >> 5] = (uint8_t)vb;
-    }
-  }
-  if (vec) {
-    store_vec(p + threadIdx.x * 16, pv);
-    if (kMaster) store_vec(wp + threadIdx.x * 16, wv);
-  } else {
-    // a thread overwrites only what it alone has read
-#pragma unroll
-    for (int j = 0; j < 16; ++j) s_w[padded(threadIdx.x * 16 + j)] = wv[j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int i = j * kThreads + threadIdx.x;
-      if (i < len) {
-        const float x = s_w[padded(i)];
-        p[i] = from_f<P>(x);
-        if (kMaster) wp[i] = x;
+      for (int j = 0; j < 16; ++j) {
+        // an element that is not finite does not set the block's exponent
+        const uint32_t a = __float_as_uint(m[j]) & 0x7fffffffu, b = __float_as_uint(v[j]) & 0x7fffffffu;
+        if (a < 0x7f800000u) mt = max(mt, a);
+        if (b < 0x7f800000u) vt = max(vt, b);
       }
+      const unsigned pair = 3u << (threadIdx.x & 30);
+      mt = max(mt, __shfl_xor_sync(pair, mt, 1));
+      vt = max(vt, __shfl_xor_sync(pair, vt, 1));
+      mb = state8::block_exp(mt, state8::kMinExpM);
+      vb = state8::block_exp(vt, state8::kMinExpV);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t r = state8::mix_folded(key ^ (uint32_t)j);
+        mq[j] = state8::encode_m(m[j], mb, state8::random_m(r));
+        vq[j] = state8::encode_v(v[j], vb, state8::random_v(r));
+      }
+    }
+    if (at < coded) {
+      *reinterpret_cast<uint4*>(mc + at) = *reinterpret_cast<uint4*>(mq);
+      *reinterpret_cast<uint4*>(vc + at) = *reinterpret_cast<uint4*>(vq);
+      if ((threadIdx.x & 1) == 0) {
+        ms[at >> 5] = (uint8_t)mb;
+        vs[at >> 5] = (uint8_t)vb;
+      }
+    }
+    if (!vec) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const unsigned i = j * kThreads + threadIdx.x;
+        if (start + i < len) {
+          const float y = s_w[padded(i)];
+          p[start + i] = from_f<P>(y);
+          if (kMaster) w[start + i] = y;
+        }
+      }
+      __syncthreads();  // the next part may be staged too
     }
   }
 }
 
 // ---------------------------------------------------------------- 8-bit states to values and back
-// 16 codes per thread (`vec`: both addresses allow 16-byte accesses), the rest one by one.
+// 16 codes per thread (`vec`: the addresses allow accesses of 16 and 32 bytes), the rest one by one.
 template <typename T, int kMoment>
 __global__ void __launch_bounds__(kThreads)
 adamw8_values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int vec, T* out) {
@@ -656,6 +765,7 @@ struct Batch {
       std::copy(tab.h, tab.h + hypers, small.h);
       small.scale = tab.scale;
       small.count = tab.count;
+      small.parts = tab.parts;
       rc = launch(small, kind, dependent, stream);
     } else {
       rc = launch(tab, kind, dependent, stream);
@@ -669,7 +779,7 @@ struct Batch {
 
   int add(const fm_adamw_group& g, int gi, int i) {
     const int64_t n = g.numels[i];
-    const int tile = g.state_bits == 8 ? kTile8 : kTile32;
+    const int tile = g.state_bits == 8 ? tab.parts * kPart8 : kTile32;
     const int64_t tiles = (n + tile - 1) / tile;
     if (tab.count > 0 && (tab.count == kLargeTable || (last_group != gi && hypers == kMaxHyper) ||
                           tab.first[tab.count] + tiles > 0x7fffffffLL)) {
@@ -695,7 +805,8 @@ struct Batch {
     e.n = n;
     e.seed = g.state_bits == 8 ? g.seeds[i] : 0;
     e.hyper = (uint16_t)(hypers - 1);
-    e.vec = aligned(e.p, 16) && aligned(e.g, 16) && aligned(e.w, 16) && aligned(e.m, 16) && aligned(e.v, 16);
+    const size_t wide = g.state_bits == 8 ? 16 : 32;  // of the moments
+    e.vec = aligned(e.p, 32) && aligned(e.g, 32) && aligned(e.w, 32) && aligned(e.m, wide) && aligned(e.v, wide);
     tab.first[tab.count + 1] = tab.first[tab.count] + (unsigned)tiles;
     ++tab.count;
     return FM_OK;
@@ -725,6 +836,13 @@ int count_steps(const fm_adamw_group* groups, int ngroups, const float* scale, c
   return flush();
 }
 
+// Parts of a tile with 8-bit states: what a block spends on its tensor's coefficients is shared by up to
+// 8 of them once that leaves every SM two rounds of blocks (8 are resident).
+int parts_of(long long elements) {
+  const long long parts = elements / ((long long)kPart8 * 12 * sm_count() + 1);
+  return parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : (int)parts;
+}
+
 int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cudaStream_t stream) {
   std::vector<Range> ranges;
   size_t tensors = 0;
@@ -749,6 +867,11 @@ int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cu
   for (int gi = 0; gi < ngroups; ++gi) {
     if (done[gi]) continue;
     batch.kind = kind_of(groups[gi]);
+    long long elements = 0;
+    for (int gj = gi; gj < ngroups; ++gj)
+      if (kind_of(groups[gj]) == batch.kind)
+        for (int i = 0; i < groups[gj].count; ++i) elements += groups[gj].numels[i];
+    batch.tab.parts = parts_of(elements);
     for (int gj = gi; gj < ngroups; ++gj) {
       if (done[gj] || !(kind_of(groups[gj]) == batch.kind)) continue;
       done[gj] = 1;
@@ -801,7 +924,7 @@ extern "C" int fm_adamw8_values(const void* codes, const void* scales, int64_t n
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int vec = aligned(codes, 16) && aligned(out, 16);
+  const int vec = aligned(codes, 16) && aligned(out, 32);
   const unsigned grid = (unsigned)((n + kThreads * 16 - 1) / (kThreads * 16));
   auto go = [&](auto* o) {
     using T = std::remove_pointer_t<decltype(o)>;

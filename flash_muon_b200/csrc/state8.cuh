@@ -58,13 +58,13 @@ FM_HD float pow2(int e) { return float_of((uint32_t)e << 23); }
 
 // A bijection of 32 bits built from xor-shifts and odd factors; the factors are the best of a search
 // for even avalanche (flipping any input bit flips every output bit with chance 0.50 +- 0.01).
-FM_HD uint32_t mix(uint32_t x) {
-  x ^= x >> 16;
+FM_HD uint32_t mix_folded(uint32_t x) {  // behind the first xor-shift
   x *= 0xa1c7d3e7u;
   x ^= x >> 15;
   x *= 0x2e3ad36du;
   return x ^ (x >> 16);
 }
+FM_HD uint32_t mix(uint32_t x) { return mix_folded(x ^ (x >> 16)); }
 // Key of a tensor's step: `count` is the step's number, counted from 1.
 FM_HD uint32_t step_key(uint32_t seed, uint32_t count) { return mix(mix(seed) + count); }
 // Key of the elements whose index has `hi` above bit 32.
