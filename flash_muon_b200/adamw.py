@@ -20,163 +20,32 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
 from collections.abc import Iterable, Sequence
-from operator import attrgetter
 
 import torch
 from torch import Tensor
 
-from ._lib import AdamWGroup, check, dtype_code, lib
-from .ops import _current_device, _raw_stream
+from . import _host
+from ._lib import check, dtype_code, lib
+from .ops import _raw_stream
 
 __all__ = ["AdamW", "adamw_step", "adamw8_step", "adamw8_values", "adamw8_encode", "grad_norm",
            "clip_grad_norm_"]
 
 _BLOCK = 32  # elements that share an exponent byte of an 8-bit state
 
-_dtype_of = attrgetter("dtype")
-_is_cuda = attrgetter("is_cuda")
-
 
 def _blocks(n: int) -> int:
     return -(-n // _BLOCK)
 
 
-def _addresses(tensors) -> array:
-    return array("Q", map(Tensor.data_ptr, tensors))
+# The entries that take lists of tensors are called through ``_host``, which checks the tensors and
+# fills the library's arrays.
+(_STEP, _NORM, _NORM_BYTES, _SCALE, _VALUES) = (
+    ctypes.cast(fn, ctypes.c_void_p).value for fn in
+    (lib.fm_adamw_step, lib.fm_grad_norm, lib.fm_grad_norm_workspace_bytes, lib.fm_scale_multi, lib.fm_adamw8_values))
 
 
-def _where(a: array | None):
-    """Address of a host array's items (the array has to outlive the call)."""
-    return a.buffer_info()[0] if a is not None else None
-
-
-def _check_tensors(name: str, tensors: Sequence[Tensor], device: int) -> None:
-    assert all(map(_is_cuda, tensors)), f"`{name}` must be CUDA tensors"
-    assert all(map(Tensor.is_contiguous, tensors)), f"`{name}` must be contiguous"
-    assert set(map(Tensor.get_device, tensors)) <= {device}, f"`{name}` must be on the parameters' device"
-
-
-def _check_numels(name: str, tensors: Sequence[Tensor], numels: list[int]) -> None:
-    assert list(map(Tensor.numel, tensors)) == numels, f"`{name}` must have the parameters' sizes"
-
-
-def _check_dtype(name: str, tensors: Sequence[Tensor], dtype: torch.dtype) -> None:
-    assert set(map(_dtype_of, tensors)) <= {dtype}, f"`{name}` must be {dtype}"
-
-
-def _check_scalar(name: str, t: Tensor, device: int) -> None:
-    assert t.is_cuda and t.get_device() == device and t.numel() == 1 and t.dtype == torch.float32, \
-        f"`{name}` must be a float32 scalar on the parameters' CUDA device"
-
-
-class _Group:
-    """One parameter group of a call: validated lists, to be turned into ``fm_adamw_group``s."""
-
-    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay,
-                 masters=None, scales=None, seeds=None):
-        n = len(params)
-        assert n == len(grads) == len(exp_avgs) == len(exp_avg_sqs), "lists must have one entry per parameter"
-        device = self.device = params[0].get_device()
-        numels = self.numels = list(map(Tensor.numel, params))
-        _check_tensors("params", params, device)
-        _check_tensors("grads", grads, device)
-        _check_numels("grads", grads, numels)
-        _check_tensors("exp_avgs", exp_avgs, device)
-        _check_tensors("exp_avg_sqs", exp_avg_sqs, device)
-        if scales is None:
-            _check_numels("exp_avgs", exp_avgs, numels)
-            _check_numels("exp_avg_sqs", exp_avg_sqs, numels)
-            _check_dtype("exp_avgs", exp_avgs, torch.float32)
-            _check_dtype("exp_avg_sqs", exp_avg_sqs, torch.float32)
-        else:
-            blocks = list(map(_blocks, numels))
-            padded = [b * _BLOCK for b in blocks]
-            assert n == len(scales[0]) == len(scales[1]) == len(seeds), "lists must have one entry per parameter"
-            for name, ts, sizes in (("exp_avgs", exp_avgs, padded), ("exp_avg_sqs", exp_avg_sqs, padded),
-                                    ("exp_avg_scales", scales[0], blocks), ("exp_avg_sq_scales", scales[1], blocks)):
-                _check_dtype(name, ts, torch.uint8)
-                assert list(map(Tensor.numel, ts)) == sizes, \
-                    f"`{name}` must have one byte per {'element, padded to 32' if sizes is padded else 'block of 32'}"
-            _check_tensors("exp_avg_scales", scales[0], device)
-            _check_tensors("exp_avg_sq_scales", scales[1], device)
-        if masters is not None:
-            assert n == len(masters), "lists must have one entry per parameter"
-            assert torch.float32 not in set(map(_dtype_of, params)), "float32 parameters have no master copies"
-            _check_tensors("masters", masters, device)
-            _check_numels("masters", masters, numels)
-            _check_dtype("masters", masters, torch.float32)
-        if isinstance(steps, Tensor):
-            assert steps.ndim == 1 and steps.numel() == n, "`steps` must have one count per parameter"
-            _check_tensors("steps", [steps], device)
-            _check_dtype("steps", [steps], torch.float32)
-            at = steps.data_ptr()
-            self.steps = array("Q", range(at, at + 4 * n, 4))
-        else:
-            assert len(steps) == n, "lists must have one entry per parameter"
-            _check_tensors("steps", steps, device)
-            _check_dtype("steps", steps, torch.float32)
-            assert all(t.numel() == 1 for t in steps), "`steps` must be scalars"
-            self.steps = _addresses(steps)
-        self.lr_device = None
-        if isinstance(lr, Tensor):
-            _check_scalar("lr", lr, device)
-            self.lr_device, lr = lr, 0.0
-        beta1, beta2 = betas
-        # refused here too: a captured call would otherwise fail only in the library
-        assert 0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, "betas must lie in [0, 1)"
-        assert eps >= 0.0 and math.isfinite(eps), "eps must be finite and not negative"
-        assert math.isfinite(lr) and math.isfinite(weight_decay), "lr and weight_decay must be finite"
-        self.settings = (float(lr), float(beta1), float(beta2), float(eps), float(weight_decay))
-        self.lists = (params, grads, masters, exp_avgs, exp_avg_sqs, *(scales or (None, None)))
-        self.p_dtypes = list(map(_dtype_of, params))
-        self.g_dtypes = list(map(_dtype_of, grads))
-        self.seeds = None if seeds is None else [int(s) & 0xffffffff for s in seeds]
-        self.bits = 32 if scales is None else 8
-
-    def structs(self, keep: list):
-        """``fm_adamw_group``s, one per pair of types; what they point to goes into ``keep``."""
-        kinds = list(zip(self.p_dtypes, self.g_dtypes))
-        for kind in dict.fromkeys(kinds):
-            for dt in kind:
-                dtype_code(dt)
-            rows = None if len(set(kinds)) == 1 else [i for i, k in enumerate(kinds) if k == kind]
-            pick = (lambda xs: xs) if rows is None else (lambda xs: [xs[i] for i in rows])
-            g = AdamWGroup()
-            arrays = [None if ts is None else _addresses(pick(ts)) for ts in self.lists]
-            arrays.append(self.steps if rows is None else array("Q", pick(self.steps)))
-            arrays.append(array("q", pick(self.numels)))
-            arrays.append(None if self.seeds is None else array("I", pick(self.seeds)))
-            keep.append(arrays)
-            (g.params, g.grads, g.masters, g.exp_avg, g.exp_avg_sq, g.exp_avg_scale, g.exp_avg_sq_scale,
-             g.steps, g.numels, g.seeds) = map(_where, arrays)
-            g.count, g.state_bits = len(arrays[0]), self.bits
-            g.p_dtype, g.g_dtype = dtype_code(kind[0]), dtype_code(kind[1])
-            g.lr, g.beta1, g.beta2, g.eps, g.weight_decay = self.settings
-            g.lr_device = None if self.lr_device is None else self.lr_device.data_ptr()
-            yield g
-
-
-def _launch(groups: list[_Group], grad_scale: Tensor | None) -> None:
-    device = groups[0].device
-    assert all(g.device == device for g in groups), "all parameters must be on one device"
-    if grad_scale is not None:
-        _check_scalar("grad_scale", grad_scale, device)
-    keep: list = []
-    structs = [s for g in groups for s in g.structs(keep)]
-    table = (AdamWGroup * len(structs))(*structs)
-    scale = None if grad_scale is None else grad_scale.data_ptr()
-    if device != _current_device():
-        with torch.cuda.device(device):
-            check(lib.fm_adamw_step(table, len(structs), scale, _raw_stream(device)))
-        return
-    rc = lib.fm_adamw_step(table, len(structs), scale, _raw_stream(device))
-    if rc:
-        check(rc)
-
-
-@torch.no_grad()
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                exp_avg_sqs: Sequence[Tensor], steps: Tensor | Sequence[Tensor], *, lr: float | Tensor,
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
@@ -189,13 +58,12 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     nothing is written, the counts included.  ``lr`` may be such a scalar too.  Parameters are
     bfloat16, float16 or float32; a 16-bit parameter takes gradients of its own type or float32.
     """
-    params = list(params)
-    if params:
-        _launch([_Group(params, list(grads), list(exp_avgs), list(exp_avg_sqs), steps, lr, betas, eps,
-                        weight_decay, masters)], grad_scale)
+    rc = _host.adamw_step(_STEP, ((params, grads, masters, exp_avgs, exp_avg_sqs, None, None, steps, None, lr, *betas,
+                                   eps, weight_decay),), grad_scale)
+    if rc:
+        check(rc)
 
 
-@torch.no_grad()
 def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                 exp_avg_scales: Sequence[Tensor], exp_avg_sqs: Sequence[Tensor],
                 exp_avg_sq_scales: Sequence[Tensor], steps: Tensor | Sequence[Tensor], *,
@@ -210,34 +78,22 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Seq
     function of the tensor's seed (``seeds[i]``, or ``seeds + i``), its step count and the element's
     index, so replicas that take the same step stay equal bit for bit.
     """
-    params = list(params)
-    if params:
-        if isinstance(seeds, int):
-            seeds = range(seeds, seeds + len(params))
-        _launch([_Group(params, list(grads), list(exp_avgs), list(exp_avg_sqs), steps, lr, betas, eps,
-                        weight_decay, masters, (list(exp_avg_scales), list(exp_avg_sq_scales)), seeds)], grad_scale)
-
-
-def _check_state8(codes: Tensor, scales: Tensor, moment: int) -> None:
-    assert moment in (1, 2), "moment must be 1 (exp_avg) or 2 (exp_avg_sq)"
-    assert codes.is_cuda and scales.is_cuda and codes.device == scales.device, "states must be CUDA tensors on one device"
-    assert codes.dtype == scales.dtype == torch.uint8, "states must be uint8"
-    assert codes.is_contiguous() and scales.is_contiguous(), "states must be contiguous"
-    assert codes.numel() == scales.numel() * _BLOCK, "states must have one scale per 32 codes"
+    if isinstance(seeds, int):
+        seeds = range(seeds, seeds + len(params))
+    rc = _host.adamw_step(_STEP, ((params, grads, masters, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales,
+                                   steps, seeds, lr, *betas, eps, weight_decay),), grad_scale)
+    if rc:
+        check(rc)
 
 
 def adamw8_values(codes: Tensor, scales: Tensor, *, moment: int, numel: int | None = None,
                   dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """The values that 8-bit states stand for, flat: ``moment`` 1 for ``exp_avg``, 2 for ``exp_avg_sq``;
     ``numel`` drops the padding.  bfloat16 and float32 hold them exactly."""
-    _check_state8(codes, scales, moment)
-    n = codes.numel() if numel is None else numel
-    assert 0 <= n <= codes.numel(), "`numel` exceeds the states"
-    with torch.cuda.device(codes.device):
-        out = torch.empty(n, dtype=dtype, device=codes.device)
-        check(lib.fm_adamw8_values(codes.data_ptr(), scales.data_ptr(), n, moment, out.data_ptr(),
-                                   dtype_code(dtype), _raw_stream(codes.device.index)))
-    return out
+    rc, values = _host.adamw8_values(_VALUES, codes, scales, moment, numel, dtype)
+    if rc:
+        check(rc)
+    return values
 
 
 def adamw8_encode(values: Tensor, *, moment: int) -> tuple[Tensor, Tensor]:
@@ -256,44 +112,17 @@ def adamw8_encode(values: Tensor, *, moment: int) -> tuple[Tensor, Tensor]:
 
 
 # ---------------------------------------------------------------- gradients
-def _gradient_table(grads: Sequence[Tensor]):
-    device = grads[0].get_device()
-    _check_tensors("grads", grads, device)
-    return (device, _addresses(grads), array("q", map(Tensor.numel, grads)),
-            array("i", [dtype_code(g.dtype) for g in grads]))
-
-
-@torch.no_grad()
 def grad_norm(grads: Sequence[Tensor], max_norm: float = math.inf) -> tuple[Tensor, Tensor]:
     """Euclidean norm over all elements of ``grads`` and the factor ``min(1, max_norm / (norm + 1e-6))``
     that clips them: two float32 scalars on the device, ready without a synchronisation for
     ``AdamW.step(grad_scale=...)``.  A norm that is not finite gives the factor NaN, with which a step
     is not taken.  Partial sums are added in 64 bits in a fixed order: equal inputs, equal bits."""
-    grads = list(grads)
-    assert grads, "`grads` must not be empty"
-    max_norm = float(max_norm)
-    assert max_norm >= 0.0, "`max_norm` must not be negative"
-    device, ptrs, numels, dtypes = _gradient_table(grads)
-    if device != _current_device():
-        with torch.cuda.device(device):
-            return _grad_norm(grads, ptrs, numels, dtypes, max_norm, device)
-    return _grad_norm(grads, ptrs, numels, dtypes, max_norm, device)
-
-
-def _grad_norm(grads, ptrs, numels, dtypes, max_norm, device):
-    need = int(lib.fm_grad_norm_workspace_bytes(len(grads)))
-    # the result and, behind it, the scratch; fresh memory for every call: calls on other streams, and
-    # graphs captured apart, have their own
-    mem = torch.empty(4 + need // 4, dtype=torch.float32, device=grads[0].device)
-    at = mem.data_ptr()
-    rc = lib.fm_grad_norm(_where(ptrs), _where(numels), _where(dtypes), len(grads), max_norm, at, at + 16, need,
-                          _raw_stream(device))
+    rc, norm, scale = _host.grad_norm(_NORM, _NORM_BYTES, grads, max_norm)
     if rc:
         check(rc)
-    return mem[0], mem[1]
+    return norm, scale
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float) -> Tensor:
     """Scales the gradients of ``parameters`` in place so that their norm is at most ``max_norm`` and
     returns the norm they had (``torch.nn.utils.clip_grad_norm_`` for the Euclidean norm).  Gradients
@@ -304,10 +133,9 @@ def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float) -> T
     if not grads:
         return torch.tensor(0.0)
     norm, scale = grad_norm(grads, max_norm)
-    device, ptrs, numels, dtypes = _gradient_table(grads)
-    with torch.cuda.device(device):
-        check(lib.fm_scale_multi(_where(ptrs), _where(numels), _where(dtypes), len(grads), scale.data_ptr(),
-                                 _raw_stream(device)))
+    rc = _host.scale(_SCALE, grads, scale)
+    if rc:
+        check(rc)
     return norm
 
 
@@ -375,33 +203,45 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        by_device: dict[int, list[_Group]] = {}
+        by_device: dict[int, list[tuple]] = {}
         index = 0
         for group in self.param_groups:
-            kinds: dict[tuple, list] = {}
+            kinds: dict[tuple, tuple] = {}
             for p in group["params"]:
                 index += 1
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                assert not p.grad.is_sparse, "AdamW takes no sparse gradients"
-                assert p.is_cuda, "AdamW parameters must be CUDA tensors"
                 state = self.state.get(p)
                 if not state:
+                    assert p.is_cuda, "`params` must be CUDA tensors"
                     if torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("take one step before capturing: a parameter has no state yet")
                     state = self._init_state(p, group)
-                kinds.setdefault((p.get_device(), "exp_avg_scale" in state, "master" in state), []).append((p, state, group["seed"] + index))
-            for (device, eight, masters), rows in kinds.items():
-                ps = [p for p, _, _ in rows]
-                states = [s for _, s, _ in rows]
-                by_device.setdefault(device, []).append(_Group(
-                    ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
-                    [s["step"] for s in states], group["lr"], group["betas"], group["eps"], group["weight_decay"],
-                    [s["master"] for s in states] if masters else None,
-                    ([s["exp_avg_scale"] for s in states], [s["exp_avg_sq_scale"] for s in states]) if eight else None,
-                    [i for _, _, i in rows] if eight else None))
+                eight, master = "exp_avg_scale" in state, state.get("master")
+                kind = (p.get_device(), eight, master is not None)
+                lists = kinds.get(kind)
+                if lists is None:  # params, grads, masters, moments, scales, steps, seeds
+                    lists = kinds[kind] = ([], [], None if master is None else [], [], [], [] if eight else None,
+                                           [] if eight else None, [], [] if eight else None)
+                lists[0].append(p)
+                lists[1].append(grad)
+                lists[3].append(state["exp_avg"])
+                lists[4].append(state["exp_avg_sq"])
+                lists[7].append(state["step"])
+                if master is not None:
+                    lists[2].append(master)
+                if eight:
+                    lists[5].append(state["exp_avg_scale"])
+                    lists[6].append(state["exp_avg_sq_scale"])
+                    lists[8].append(group["seed"] + index)
+            for kind, lists in kinds.items():
+                by_device.setdefault(kind[0], []).append(
+                    (*lists, group["lr"], *group["betas"], group["eps"], group["weight_decay"]))
         for groups in by_device.values():
-            _launch(groups, grad_scale)
+            rc = _host.adamw_step(_STEP, groups, grad_scale)
+            if rc:
+                check(rc)
         return loss
 
     def state_values(self, p: Tensor) -> tuple[Tensor, Tensor]:
