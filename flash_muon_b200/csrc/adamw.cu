@@ -27,8 +27,9 @@ constexpr int kTile32 = 1024;      // elements of a block, 8 per thread, with 32
 constexpr int kPart8 = 2048;       // 16 per thread with 8-bit states, where two threads share a block of
 constexpr int kMaxParts = 8;       // 32, and a block takes up to 8 such parts
 constexpr int kMaxHyper = 8;       // parameter groups of one launch
-constexpr int kSmallTable = 40;    // tensors of one launch: the table travels as a kernel argument,
-constexpr int kLargeTable = 360;   // small (4 KB) where it suffices, else up to the limit of 32764 bytes
+// Tensors of one launch.  The table travels as a kernel argument, of 3, 9 or 30 KB (the limit is 32764
+// bytes): the largest costs the host 1.4 us more per launch than the smallest.
+constexpr int kSmallTable = 24, kMediumTable = 96, kLargeTable = 360;
 constexpr int kCountTable = 480;
 
 struct Entry {
@@ -303,6 +304,20 @@ __device__ __forceinline__ uint32_t at_most_inf(uint32_t h2) {
   asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h2), "r"(0x7c007c00u));
   return r;
 }
+// Codes of a word (the upper two where `upper`) without their block's factor, and the factors:
+// 2^(b - 134) and 2^(b - 141) times the codes read as e4m3 and f16.  Fresh states have scale byte 0 and
+// only zero codes.
+__device__ __forceinline__ f32x2 decode_m2(uint32_t w, bool upper) {
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((unsigned short)(upper ? w >> 16 : w)));
+  return halves_to_floats(h2);
+}
+__device__ __forceinline__ f32x2 decode_v2(uint32_t w, bool upper) {
+  // code 255, infinity, comes out of the shift as "not a number"
+  return halves_to_floats(at_most_inf(__byte_perm(w, 0, upper ? 0x4342 : 0x4140) << 7));
+}
+__device__ __forceinline__ float factor_m(int b) { return state8::pow2(max(b, state8::kMinExpM) - 7); }
+__device__ __forceinline__ float factor_v(int b) { return state8::pow2(max(b, state8::kMinExpV) - 14); }
 // A word of padding per 16: a thread's 16 elements and a warp's neighbouring ones are both free of
 // bank conflicts.
 __device__ __forceinline__ int padded(int i) { return i + (i >> 4); }
@@ -459,17 +474,11 @@ __global__ void __launch_bounds__(kThreads, 6) adamw8_kernel(const __grid_consta
 
     float m[16], v[16];
     alignas(16) float wn[16];
-    // 2^(b - 134) and 2^(b - 141) times the codes read as e4m3 and f16; a scale byte of 0 (fresh
-    // states) has only zero codes
-    const f32x2 mf = both(state8::pow2(max(mb, state8::kMinExpM) - 7)), vf = both(state8::pow2(max(vb, state8::kMinExpV) - 14));
+    const f32x2 mf = both(factor_m(mb)), vf = both(factor_v(vb));
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
-      const uint32_t mw = reinterpret_cast<uint32_t*>(mq)[j / 4], vw = reinterpret_cast<uint32_t*>(vq)[j / 4];
-      uint32_t mh;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(mh) : "h"((unsigned short)(j & 2 ? mw >> 16 : mw)));
-      f32x2 m2 = mul2(halves_to_floats(mh), mf);
-      // code 255, infinity, comes out of the shift as "not a number"
-      f32x2 v2 = mul2(halves_to_floats(at_most_inf(__byte_perm(vw, 0, j & 2 ? 0x4342 : 0x4140) << 7)), vf);
+      f32x2 m2 = mul2(decode_m2(reinterpret_cast<uint32_t*>(mq)[j / 4], j & 2), mf);
+      f32x2 v2 = mul2(decode_v2(reinterpret_cast<uint32_t*>(vq)[j / 4], j & 2), vf);
       const f32x2 g2 = mul2(pack2(to_f<G>(gv[j]), to_f<G>(gv[j + 1])), sc);
       m2 = fma2(b1, m2, mul2(o1, g2));
       v2 = fma2(b2, v2, mul2(o2, mul2(g2, g2)));
@@ -586,24 +595,34 @@ __global__ void __launch_bounds__(kThreads, 6) adamw8_kernel(const __grid_consta
 }
 
 // ---------------------------------------------------------------- 8-bit states to values and back
-// 16 codes per thread (`vec`: the addresses allow accesses of 16 and 32 bytes), the rest one by one.
+// A block of 32 codes per thread (`vec`: the addresses allow accesses of 32 bytes), else one by one.
 template <typename T, int kMoment>
 __global__ void __launch_bounds__(kThreads)
 adamw8_values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int vec, T* out) {
-  const long long at = ((long long)blockIdx.x * kThreads + threadIdx.x) * 16;
+  const long long at = ((long long)blockIdx.x * kThreads + threadIdx.x) * 32;
   if (at >= n) return;
   const int b = exps[at >> 5];
-  auto value = [&](uint8_t c) { return kMoment == 1 ? state8::decode_m(c, b) : state8::decode_v(c, b); };
-  if (vec && at + 16 <= n) {
-    alignas(16) uint8_t c[16];
-    alignas(16) T x[16];
-    *reinterpret_cast<uint4*>(c) = *reinterpret_cast<const uint4*>(codes + at);
+  if (vec && at + 32 <= n) {
+    alignas(32) uint8_t c[32];
+    load_vec(codes + at, c);
+    const f32x2 factor = both(kMoment == 1 ? factor_m(b) : factor_v(b));
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = from_f<T>(value(c[j]));
-    store_vec(out + at, x);
+    for (int h = 0; h < 2; ++h) {  // 16 at a time: fewer registers
+      alignas(32) T x[16];
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(c)[(16 * h + j) / 4];
+        float lo, hi;
+        unpack2(mul2(kMoment == 1 ? decode_m2(w, j & 2) : decode_v2(w, j & 2), factor), lo, hi);
+        x[j] = from_f<T>(lo);
+        x[j + 1] = from_f<T>(hi);
+      }
+      store_vec(out + at + 16 * h, x);
+    }
     return;
   }
-  for (int j = 0; j < 16 && at + j < n; ++j) out[at + j] = from_f<T>(value(codes[at + j]));
+  for (int j = 0; j < 32 && at + j < n; ++j)
+    out[at + j] = from_f<T>(kMoment == 1 ? state8::decode_m(codes[at + j], b) : state8::decode_v(codes[at + j], b));
 }
 
 // One warp per block of 32, rounding to nearest.
@@ -632,8 +651,15 @@ struct Range {
 };
 
 // Refuses a call whose written memory overlaps anything else of the call: two threads would race.
-int check_ranges(std::vector<Range>& r) {
-  std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+// `runs`: where each list of tensors begins in r.  Lists are mostly in the order of their addresses
+// already, and merging sorted lists is several times cheaper than sorting.
+int check_ranges(std::vector<Range>& r, const std::vector<size_t>& runs) {
+  const auto less = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  for (size_t i = 0; i < runs.size(); ++i) {
+    const auto from = r.begin() + runs[i], to = i + 1 < runs.size() ? r.begin() + runs[i + 1] : r.end();
+    if (!std::is_sorted(from, to, less)) std::sort(from, to, less);
+    std::inplace_merge(r.begin(), from, to, less);
+  }
   uintptr_t any = 0, written = 0;
   for (const Range& x : r) {
     if (x.begin < (x.written ? any : written))
@@ -644,7 +670,7 @@ int check_ranges(std::vector<Range>& r) {
   return FM_OK;
 }
 
-int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges) {
+int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges, std::vector<size_t>& runs) {
   if (g.count < 0) return fail(FM_ERR_INVALID, "group %d: negative count", gi);
   if (g.count == 0) return FM_OK;
   if (!g.params || !g.grads || !g.exp_avg || !g.exp_avg_sq || !g.steps || !g.numels)
@@ -669,29 +695,38 @@ int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges) {
     const int64_t n = g.numels[i];
     if (n < 0 || n > (int64_t)1 << 38) return fail(FM_ERR_INVALID, "group %d: bad element count at %d", gi, i);
     if (!g.steps[i] || !aligned(g.steps[i], 4)) return fail(FM_ERR_INVALID, "group %d: bad step count at %d", gi, i);
-    ranges.push_back({(uintptr_t)g.steps[i], (uintptr_t)g.steps[i] + 4, true});
     if (n == 0) continue;
     if (!g.params[i] || !g.grads[i] || !g.exp_avg[i] || !g.exp_avg_sq[i] || (g.masters && !g.masters[i]))
       return fail(FM_ERR_INVALID, "group %d: null tensor pointer at %d", gi, i);
     if (!aligned(g.params[i], pb) || !aligned(g.grads[i], gb) || (g.masters && !aligned(g.masters[i], 4)) ||
         !aligned(g.exp_avg[i], g.state_bits == 8 ? 16 : 4) || !aligned(g.exp_avg_sq[i], g.state_bits == 8 ? 16 : 4))
       return fail(FM_ERR_INVALID, "group %d: misaligned tensor at %d", gi, i);
-    const size_t ns = g.state_bits == 8 ? (size_t)(n + 31) / 32 * 32 : (size_t)n;
-    auto add = [&](const void* q, size_t bytes, bool written) {
-      ranges.push_back({(uintptr_t)q, (uintptr_t)q + bytes, written});
-    };
-    add(g.params[i], n * pb, true);
-    add(g.grads[i], n * gb, false);
-    add(g.exp_avg[i], ns * sb, true);
-    add(g.exp_avg_sq[i], ns * sb, true);
-    if (g.masters) add(g.masters[i], n * 4, true);
-    if (g.state_bits == 8) {
-      if (!g.exp_avg_scale[i] || !g.exp_avg_sq_scale[i])
-        return fail(FM_ERR_INVALID, "group %d: null scales at %d", gi, i);
-      add(g.exp_avg_scale[i], ns / 32, true);
-      add(g.exp_avg_sq_scale[i], ns / 32, true);
-    }
+    if (g.state_bits == 8 && (!g.exp_avg_scale[i] || !g.exp_avg_sq_scale[i]))
+      return fail(FM_ERR_INVALID, "group %d: null scales at %d", gi, i);
   }
+  // `unit` bytes per element, or per block of 32 where `blocks`
+  auto add = [&](auto* list, size_t unit, bool written, bool padded, bool blocks) {
+    runs.push_back(ranges.size());
+    for (int i = 0; i < g.count; ++i) {
+      size_t n = (size_t)g.numels[i];
+      if (n == 0) continue;
+      if (padded || blocks) n = (n + 31) / 32 * (blocks ? 1 : 32);
+      const uintptr_t at = (uintptr_t)list[i];
+      ranges.push_back({at, at + n * unit, written});
+    }
+  };
+  const bool eight = g.state_bits == 8;
+  add(g.params, pb, true, false, false);
+  add(g.grads, gb, false, false, false);
+  add(g.exp_avg, sb, true, eight, false);
+  add(g.exp_avg_sq, sb, true, eight, false);
+  if (g.masters) add(g.masters, 4, true, false, false);
+  if (eight) {
+    add(g.exp_avg_scale, 1, true, false, true);
+    add(g.exp_avg_sq_scale, 1, true, false, true);
+  }
+  runs.push_back(ranges.size());
+  for (int i = 0; i < g.count; ++i) ranges.push_back({(uintptr_t)g.steps[i], (uintptr_t)g.steps[i] + 4, true});
   return FM_OK;
 }
 
@@ -755,21 +790,24 @@ struct Batch {
   bool dependent = false;  // the next launch follows the counts directly
   cudaStream_t stream;
 
+  template <int N>
+  int launch_part() {
+    Table<N> t;
+    std::copy(tab.e, tab.e + tab.count, t.e);
+    std::copy(tab.first, tab.first + tab.count + 1, t.first);
+    std::copy(tab.h, tab.h + hypers, t.h);
+    t.scale = tab.scale;
+    t.count = tab.count;
+    t.parts = tab.parts;
+    return launch(t, kind, dependent, stream);
+  }
+
   int flush() {
     if (tab.count == 0) return FM_OK;
     int rc;
-    if (tab.count <= kSmallTable) {
-      Table<kSmallTable> small;
-      std::copy(tab.e, tab.e + tab.count, small.e);
-      std::copy(tab.first, tab.first + tab.count + 1, small.first);
-      std::copy(tab.h, tab.h + hypers, small.h);
-      small.scale = tab.scale;
-      small.count = tab.count;
-      small.parts = tab.parts;
-      rc = launch(small, kind, dependent, stream);
-    } else {
-      rc = launch(tab, kind, dependent, stream);
-    }
+    if (tab.count <= kSmallTable) rc = launch_part<kSmallTable>();
+    else if (tab.count <= kMediumTable) rc = launch_part<kMediumTable>();
+    else rc = launch(tab, kind, dependent, stream);
     tab.count = 0;
     hypers = 0;
     last_group = -1;
@@ -848,13 +886,15 @@ int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cu
   size_t tensors = 0;
   for (int gi = 0; gi < ngroups; ++gi) tensors += groups[gi].count > 0 ? groups[gi].count : 0;
   ranges.reserve(tensors * 8);
+  std::vector<size_t> runs;
+  runs.reserve(ngroups * 8);
   for (int gi = 0; gi < ngroups; ++gi) {
-    const int rc = check_group(groups[gi], gi, ranges);
+    const int rc = check_group(groups[gi], gi, ranges, runs);
     if (rc != FM_OK) return rc;
   }
   if (tensors == 0) return FM_OK;
   if (!aligned(scale, 4)) return fail(FM_ERR_INVALID, "misaligned gradient scale");
-  int rc = check_ranges(ranges);
+  int rc = check_ranges(ranges, runs);
   if (rc != FM_OK) return rc;
   rc = count_steps(groups, ngroups, scale, stream);
   if (rc != FM_OK) return rc;
@@ -924,8 +964,8 @@ extern "C" int fm_adamw8_values(const void* codes, const void* scales, int64_t n
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int vec = aligned(codes, 16) && aligned(out, 32);
-  const unsigned grid = (unsigned)((n + kThreads * 16 - 1) / (kThreads * 16));
+  const int vec = aligned(codes, 32) && aligned(out, 32);
+  const unsigned grid = (unsigned)((n + kThreads * 32 - 1) / (kThreads * 32));
   auto go = [&](auto* o) {
     using T = std::remove_pointer_t<decltype(o)>;
     if (moment == 1) adamw8_values_kernel<T, 1><<<grid, kThreads, 0, st>>>(c, s, n, vec, o);
