@@ -23,9 +23,11 @@ namespace fm {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kTile32 = 1024;      // elements of a block, 8 per thread, with 32-bit states
+constexpr int kEach32 = 8;         // elements per thread with 32-bit states: a tile of 1024
+constexpr int kMaxThreads = 1024;  // of a block that takes a whole small tensor
 constexpr int kPart8 = 2048;       // 16 per thread with 8-bit states, where two threads share a block of
 constexpr int kMaxParts = 8;       // 32, and a block takes up to 8 such parts
+constexpr int kWholeParts = 4;     // parts of a whole small tensor
 constexpr int kMaxHyper = 8;       // parameter groups of one launch
 // Tensors of one launch.  The table travels as a kernel argument, of 3, 9 or 30 KB (the limit is 32764
 // bytes): the largest costs the host 1.4 us more per launch than the smallest.
@@ -40,7 +42,7 @@ struct Entry {
   void* v;
   uint8_t* ms;       // exponent bytes, 8-bit states only
   uint8_t* vs;
-  const float* step;
+  float* step;
   long long n;
   uint32_t seed;
   uint16_t hyper;
@@ -59,6 +61,8 @@ struct Table {
   const float* scale;
   int count;
   int parts;              // 8-bit states: parts of a tile
+  int threads;            // 32-bit states: threads of a block
+  int whole;              // every tensor has one block, which advances its count
 };
 struct CountTable {
   float* step[kCountTable];
@@ -149,11 +153,14 @@ __device__ __forceinline__ int find(const Tab& tab, unsigned tile) {
 // The coefficients of the block's tensor, one per warp's first thread, behind the loads of its tile:
 // reading the count and the powers (17 dependent 64-bit products at t = 100000) take less than the
 // loads do.
-__device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, uint32_t index_hi, Coef* c) {
+__device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, uint32_t index_hi, bool whole, bool taken,
+                                             Coef* c) {
   // the counts are the previous launch's
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  float count = 0.f;
   if ((threadIdx.x & 31) == 0) {
-    const unsigned t = (unsigned)*reinterpret_cast<const volatile float*>(e.step);
+    count = *reinterpret_cast<const volatile float*>(e.step) + (whole ? 1.f : 0.f);
+    const unsigned t = (unsigned)count;
     const int which = threadIdx.x >> 5;
     if (which == 0) {
       const float lr = h.lr_dev ? *h.lr_dev : (float)h.lr;
@@ -162,17 +169,19 @@ __device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, uin
       c->root = 1.f / sqrtf((float)(1.0 - power(h.beta2, t)));
     } else if (which == 2) {
       c->key = state8::index_key(state8::step_key(e.seed, t), index_hi);
-    } else {
+    } else if (which == 3) {
       c->decay = (float)(1.0 - (h.lr_dev ? (double)*h.lr_dev : h.lr) * h.wd);
     }
   }
   __syncthreads();
+  if (whole && taken && threadIdx.x == 0) *e.step = count;  // read by all of its readers
 }
 
 // ---------------------------------------------------------------- step counts
 // The counts are advanced by a launch of their own ahead of the step's: every block of the step
 // reads its tensor's count, so none of them may write it.  The step's blocks start while it runs
-// and load their tiles: all that those hold was written before this launch began.
+// and load their tiles: all that those hold was written before this launch began.  Where all
+// tensors of a kind are small a block takes each of them whole and advances its count itself.
 __global__ void __launch_bounds__(kThreads) adamw_count_kernel(const __grid_constant__ CountTable tab) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (skipped(tab.scale)) return;
@@ -180,20 +189,22 @@ __global__ void __launch_bounds__(kThreads) adamw_count_kernel(const __grid_cons
 }
 
 // ---------------------------------------------------------------- states in fp32
-template <typename P, typename G, bool kMaster, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> tab) {
+// kWhole: a block of up to 1024 threads takes a whole tensor.
+template <typename P, typename G, bool kMaster, bool kWhole, int N>
+__global__ void __launch_bounds__(kWhole ? kMaxThreads : kThreads) adamw_kernel(const __grid_constant__ Table<N> tab) {
   __shared__ Coef s_coef;
   const int ti = find(tab, blockIdx.x);
   const Entry& e = tab.e[ti];
   const Hyper& h = tab.h[e.hyper];
-  const long long base = (long long)(blockIdx.x - tab.first[ti]) * kTile32;
+  const int threads = kWhole ? blockDim.x : kThreads, tile = threads * kEach32;
+  const long long base = (long long)(blockIdx.x - tab.first[ti]) * tile;
   P* const p = static_cast<P*>(e.p) + base;
   const G* const g = static_cast<const G*>(e.g) + base;
   float* const w = e.w + base;
   float* const m = static_cast<float*>(e.m) + base;
   float* const v = static_cast<float*>(e.v) + base;
-  const bool vec = e.vec && base + kTile32 <= e.n;
-  const int len = (int)(e.n - base < kTile32 ? e.n - base : kTile32);
+  const bool vec = e.vec && base + tile <= e.n;
+  const int len = (int)(e.n - base < tile ? e.n - base : tile);
   alignas(16) P pv[8];
   alignas(16) G gv[8];
   alignas(16) float mv[8], vv[8], wv[8];
@@ -204,10 +215,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     load_vec(g + at, gv);
     load_vec(m + at, mv);
     load_vec(v + at, vv);
-  } else {    // 8 elements kThreads apart
+  } else {    // 8 elements `threads` apart
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int at = j * kThreads + threadIdx.x;
+      const int at = j * threads + threadIdx.x;
       const bool here = at < len;
       if (kMaster) wv[j] = here ? w[at] : 0.f;
       else pv[j] = here ? p[at] : from_f<P>(0.f);
@@ -217,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     }
   }
   const float scale = tab.scale ? *tab.scale : 1.f;
-  coefficients(h, e, 0, &s_coef);
+  coefficients(h, e, 0, kWhole, finite(scale), &s_coef);
   if (!finite(scale)) return;
   const Coef c = s_coef;
 #pragma unroll
@@ -237,7 +248,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int at = j * kThreads + threadIdx.x;
+      const int at = j * threads + threadIdx.x;
       if (at < len) {
         p[at] = pv[j];
         if (kMaster) w[at] = wv[j];
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 6) adamw8_kernel(const __grid_consta
       }
     }
     if (start == 0) {
-      coefficients(h, e, (uint32_t)(base >> 32), &s_coef);
+      coefficients(h, e, (uint32_t)(base >> 32), tab.whole, finite(scale), &s_coef);
       if (!finite(scale)) {
         copy_wait<0>();
         return;
@@ -742,7 +753,7 @@ template <auto kernel, typename Tab>
 int launch_table(const Tab& tab, bool dependent, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tab.first[tab.count]);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(tab.threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -756,7 +767,8 @@ int launch_table(const Tab& tab, bool dependent, cudaStream_t stream) {
 template <typename P, typename G, bool kMaster, int N>
 int launch_kind(const Table<N>& tab, int bits, bool dependent, cudaStream_t stream) {
   if (bits == 8) return launch_table<adamw8_kernel<P, G, kMaster, N>>(tab, dependent, stream);
-  return launch_table<adamw_kernel<P, G, kMaster, N>>(tab, dependent, stream);
+  if (tab.whole) return launch_table<adamw_kernel<P, G, kMaster, true, N>>(tab, dependent, stream);
+  return launch_table<adamw_kernel<P, G, kMaster, false, N>>(tab, dependent, stream);
 }
 
 template <int N>
@@ -799,6 +811,8 @@ struct Batch {
     t.scale = tab.scale;
     t.count = tab.count;
     t.parts = tab.parts;
+    t.threads = tab.threads;
+    t.whole = tab.whole;
     return launch(t, kind, dependent, stream);
   }
 
@@ -817,7 +831,7 @@ struct Batch {
 
   int add(const fm_adamw_group& g, int gi, int i) {
     const int64_t n = g.numels[i];
-    const int tile = g.state_bits == 8 ? tab.parts * kPart8 : kTile32;
+    const int tile = g.state_bits == 8 ? tab.parts * kPart8 : tab.threads * kEach32;
     const int64_t tiles = (n + tile - 1) / tile;
     if (tab.count > 0 && (tab.count == kLargeTable || (last_group != gi && hypers == kMaxHyper) ||
                           tab.first[tab.count] + tiles > 0x7fffffffLL)) {
@@ -851,35 +865,31 @@ struct Batch {
   }
 };
 
-int count_steps(const fm_adamw_group* groups, int ngroups, const float* scale, cudaStream_t stream) {
-  CountTable tab;
-  tab.scale = scale;
-  tab.count = 0;
-  auto flush = [&]() -> int {
-    if (tab.count == 0) return FM_OK;
-    adamw_count_kernel<<<1, kThreads, 0, stream>>>(tab);
-    tab.count = 0;
-    FM_CUDA_CHECK(cudaGetLastError());
-    return FM_OK;
-  };
-  for (int gi = 0; gi < ngroups; ++gi) {
-    for (int i = 0; i < groups[gi].count; ++i) {
-      tab.step[tab.count++] = groups[gi].steps[i];
-      if (tab.count == kCountTable) {
-        const int rc = flush();
-        if (rc != FM_OK) return rc;
-      }
-    }
-  }
-  return flush();
-}
-
 // Parts of a tile with 8-bit states: what a block spends on its tensor's coefficients is shared by up to
 // 8 of them once that leaves every SM two rounds of blocks (8 are resident).
 int parts_of(long long elements) {
   const long long parts = elements / ((long long)kPart8 * 12 * sm_count() + 1);
   return parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : (int)parts;
 }
+
+// The counts of what is added, advanced by as many launches as that takes.
+struct Counts {
+  CountTable tab;
+  cudaStream_t stream;
+  bool launched = false;
+  int add(float* step) {
+    tab.step[tab.count++] = step;
+    return tab.count == kCountTable ? flush() : FM_OK;
+  }
+  int flush() {
+    if (tab.count == 0) return FM_OK;
+    adamw_count_kernel<<<1, kThreads, 0, stream>>>(tab);
+    tab.count = 0;
+    launched = true;
+    FM_CUDA_CHECK(cudaGetLastError());
+    return FM_OK;
+  }
+};
 
 int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cudaStream_t stream) {
   std::vector<Range> ranges;
@@ -896,33 +906,70 @@ int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cu
   if (!aligned(scale, 4)) return fail(FM_ERR_INVALID, "misaligned gradient scale");
   int rc = check_ranges(ranges, runs);
   if (rc != FM_OK) return rc;
-  rc = count_steps(groups, ngroups, scale, stream);
+
+  // the kinds of the call, their elements and largest tensors
+  struct Work {
+    Kind kind;
+    long long elements = 0, largest = 0;
+  };
+  std::vector<Work> works;
+  std::vector<int> work_of(ngroups, 0);
+  for (int gi = 0; gi < ngroups; ++gi) {
+    const Kind k = kind_of(groups[gi]);
+    size_t w = 0;
+    while (w < works.size() && !(works[w].kind == k)) ++w;
+    if (w == works.size()) works.push_back({k});
+    work_of[gi] = (int)w;
+    for (int i = 0; i < groups[gi].count; ++i) {
+      works[w].elements += groups[gi].numels[i];
+      works[w].largest = std::max(works[w].largest, (long long)groups[gi].numels[i]);
+    }
+  }
+  // One block per tensor saves the launch of the counts, 2 us, as long as a block is not much longer
+  // over a tensor than many blocks are: up to 8192 elements.
+  const auto whole = [&](const Work& w) {
+    return w.largest <= (w.kind.bits == 8 ? kWholeParts * kPart8 : kMaxThreads * kEach32);
+  };
+  Counts counts;
+  counts.tab.count = 0;
+  counts.tab.scale = scale;
+  counts.stream = stream;
+  for (int gi = 0; gi < ngroups; ++gi) {
+    const bool all = !whole(works[work_of[gi]]);
+    for (int i = 0; i < groups[gi].count && rc == FM_OK; ++i)
+      if (all || groups[gi].numels[i] == 0) rc = counts.add(groups[gi].steps[i]);
+  }
+  if (rc == FM_OK) rc = counts.flush();
   if (rc != FM_OK) return rc;
+
   Batch batch;
   batch.tab.count = 0;
   batch.tab.scale = scale;
   batch.stream = stream;
-  batch.dependent = options().pdl != 0;
-  std::vector<char> done(ngroups, 0);
-  for (int gi = 0; gi < ngroups; ++gi) {
-    if (done[gi]) continue;
-    batch.kind = kind_of(groups[gi]);
-    long long elements = 0;
-    for (int gj = gi; gj < ngroups; ++gj)
-      if (kind_of(groups[gj]) == batch.kind)
-        for (int i = 0; i < groups[gj].count; ++i) elements += groups[gj].numels[i];
-    batch.tab.parts = parts_of(elements);
-    for (int gj = gi; gj < ngroups; ++gj) {
-      if (done[gj] || !(kind_of(groups[gj]) == batch.kind)) continue;
-      done[gj] = 1;
-      for (int i = 0; i < groups[gj].count; ++i) {
-        if (groups[gj].numels[i] == 0) continue;
-        rc = batch.add(groups[gj], gj, i);
-        if (rc != FM_OK) return rc;
+  batch.dependent = counts.launched && options().pdl != 0;
+  for (const bool now : {false, true}) {  // what waits for the counts follows them directly
+    for (size_t w = 0; w < works.size(); ++w) {
+      const Work& work = works[w];
+      if (whole(work) != now || work.elements == 0) continue;
+      batch.kind = work.kind;
+      batch.tab.whole = now;
+      batch.tab.threads = kThreads;
+      batch.tab.parts = parts_of(work.elements);
+      if (now) {
+        batch.tab.parts = (int)((work.largest + kPart8 - 1) / kPart8);
+        while (work.kind.bits == 32 && batch.tab.threads * kEach32 < work.largest) batch.tab.threads *= 2;
       }
+      for (int gi = 0; gi < ngroups; ++gi) {
+        if (work_of[gi] != (int)w) continue;
+        for (int i = 0; i < groups[gi].count; ++i) {
+          if (groups[gi].numels[i] == 0) continue;
+          rc = batch.add(groups[gi], gi, i);
+          if (rc != FM_OK) return rc;
+        }
+      }
+      rc = batch.flush();
+      if (rc != FM_OK) return rc;
     }
-    rc = batch.flush();
-    if (rc != FM_OK) return rc;
   }
   return FM_OK;
 }
