@@ -1,5 +1,6 @@
 // Norm over all gradients of a model, the factor that clips it, and the scaling by it.  Each is one
 // pass over the gradients: the bound is HBM.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -15,6 +16,9 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 8192;         // elements a block takes at a time
 constexpr int kSmallTable = 64;      // tensors of one launch: the table travels as a kernel argument
 constexpr int kLargeTable = 1024;
+// Up to 512 units of 1024 elements, a unit per warp at a time, go to one cluster of blocks, which adds up
+// in shared memory and leaves the result itself: one launch instead of two.
+constexpr int kUnit = 1024, kMaxUnits = 512, kCluster = 8, kClusterThreads = 512;
 constexpr int kMaxBlocks = 1184;     // partial sums of one launch, 8 per SM; fixed, so that the
                                      // order of the sum is the same whatever else runs
 
@@ -35,6 +39,12 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ double warp_sum(double s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
 
 // Blocks walk contiguous ranges of the chunks of all tensors.
 template <typename Tab, typename Body>
@@ -94,8 +104,7 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   double s = 0.0;
   walk(tab, [&](auto* g, int len) { s += (double)chunk_sumsq(g, len); });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  s = warp_sum(s);
   __shared__ double red[kThreads / 32];
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
@@ -106,23 +115,94 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
   }
 }
 
+__device__ __forceinline__ void write_result(double sum, double max_norm, float* result) {
+  const float norm = (float)sqrt(sum);
+  const float ratio = (float)max_norm / (norm + 1e-6f);
+  result[0] = norm;
+  result[1] = fabsf(norm) <= 3.402823466e38f ? fminf(ratio, 1.f) : __int_as_float(0x7fc00000);
+}
+
+// Sum of a lane's 32 squares of a unit of `len` elements.
+template <typename T>
+__device__ __forceinline__ float unit_sumsq(const T* g, int len) {
+  constexpr int V = 16 / sizeof(T), L = kUnit / (32 * V);
+  const int lane = threadIdx.x & 31;
+  float s = 0.f;
+  if (len == kUnit && (reinterpret_cast<uintptr_t>(g) & 15u) == 0) {
+    uint4 raw[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(g) + i * 32 + lane);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const T* e = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float f = to_f<T>(e[j]);
+        s = fmaf(f, f, s);
+      }
+    }
+    return s;
+  }
+#pragma unroll 8
+  for (int i = lane; i < len; i += 32) {
+    const float f = to_f<T>(g[i]);
+    s = fmaf(f, f, s);
+  }
+  return s;
+}
+
+template <int N>
+__global__ void __cluster_dims__(kCluster) __launch_bounds__(kClusterThreads)
+grad_norm_small_kernel(const __grid_constant__ Table<N> tab, double max_norm, float* result) {
+  namespace cg = cooperative_groups;
+  __shared__ double red[kClusterThreads / 32], all[kCluster];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const unsigned total = tab.first[tab.count];
+  const int warp = threadIdx.x >> 5;
+  double s = 0.0;
+  for (unsigned u = warp * kCluster + blockIdx.x; u < total; u += kCluster * (kClusterThreads / 32)) {
+    int lo = 0, hi = tab.count;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tab.first[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    const long long base = (long long)(u - tab.first[lo]) * kUnit, left = tab.n[lo] - base;
+    const int len = (int)(left < kUnit ? left : kUnit);
+    switch (tab.dtype[lo]) {
+      case FM_BF16: s += (double)unit_sumsq(static_cast<__nv_bfloat16*>(tab.g[lo]) + base, len); break;
+      case FM_F16: s += (double)unit_sumsq(static_cast<__half*>(tab.g[lo]) + base, len); break;
+      default: s += (double)unit_sumsq(static_cast<float*>(tab.g[lo]) + base, len); break;
+    }
+  }
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) red[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kClusterThreads / 32; ++i) s += red[i];
+    cluster.map_shared_rank(all, 0)[blockIdx.x] = s;
+  }
+  cluster.sync();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    s = all[0];
+    for (int i = 1; i < kCluster; ++i) s += all[i];
+    write_result(s, max_norm, result);
+  }
+}
+
 __global__ void __launch_bounds__(kThreads)
 grad_norm_result_kernel(const double* partials, int count, double max_norm, float* result) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   double s = 0.0;
   for (int i = threadIdx.x; i < count; i += kThreads) s += partials[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  s = warp_sum(s);
   __shared__ double red[kThreads / 32];
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     s = red[0];
     for (int i = 1; i < kThreads / 32; ++i) s += red[i];
-    const float norm = (float)sqrt(s);
-    const float ratio = (float)max_norm / (norm + 1e-6f);
-    result[0] = norm;
-    result[1] = fabsf(norm) <= 3.402823466e38f ? fminf(ratio, 1.f) : __int_as_float(0x7fc00000);
+    write_result(s, max_norm, result);
   }
 }
 
@@ -165,13 +245,13 @@ int check_tensors(const void* const* grads, const int64_t* numels, const int32_t
 
 // Fills tables and hands each to `go(table)`.
 template <int N, typename Go>
-int for_tables(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, Go go) {
+int for_tables(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, int chunk, Go go) {
   Table<N> tab;
   tab.count = 0;
   tab.first[0] = 0;
   for (int i = 0; i < count; ++i) {
     if (numels[i] == 0) continue;
-    const long long chunks = (numels[i] + kChunk - 1) / kChunk;
+    const long long chunks = (numels[i] + chunk - 1) / chunk;
     if (tab.count == N || tab.first[tab.count] + chunks > 0x7fffffffLL) {
       const int rc = go(tab);
       if (rc != FM_OK) return rc;
@@ -221,8 +301,20 @@ extern "C" int fm_grad_norm(const void* const* grads, const int64_t* numels, con
     FM_CUDA_CHECK(cudaGetLastError());
     return FM_OK;
   };
-  rc = count <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, go)
-                            : for_tables<kLargeTable>(grads, numels, dtypes, count, go);
+  long long units = 0;
+  for (int i = 0; i < count; ++i) units += (numels[i] + kUnit - 1) / kUnit;
+  if (units > 0 && units <= kMaxUnits) {
+    auto all = [&](const auto& tab) -> int {
+      grad_norm_small_kernel<<<kCluster, kClusterThreads, 0, st>>>(tab, max_norm, result);
+      FM_CUDA_CHECK(cudaGetLastError());
+      return FM_OK;
+    };
+    // every tensor that is not empty has a unit: one table holds them all
+    return units <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, kUnit, all)
+                                : for_tables<kMaxUnits>(grads, numels, dtypes, count, kUnit, all);
+  }
+  rc = count <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, kChunk, go)
+                            : for_tables<kLargeTable>(grads, numels, dtypes, count, kChunk, go);
   if (rc != FM_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1);
@@ -252,6 +344,6 @@ extern "C" int fm_scale_multi(void* const* grads, const int64_t* numels, const i
     FM_CUDA_CHECK(cudaGetLastError());
     return FM_OK;
   };
-  return count <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, go)
-                              : for_tables<kLargeTable>(grads, numels, dtypes, count, go);
+  return count <= kSmallTable ? for_tables<kSmallTable>(grads, numels, dtypes, count, kChunk, go)
+                              : for_tables<kLargeTable>(grads, numels, dtypes, count, kChunk, go);
 }

@@ -32,7 +32,9 @@ B16, H16, F32 = torch.bfloat16, torch.float16, torch.float32
 KINDS = [(B16, B16, False), (B16, F32, False), (H16, H16, False), (H16, F32, False), (F32, F32, False),
          (F32, B16, False), (F32, H16, False), (B16, B16, True), (B16, F32, True), (H16, H16, True), (H16, F32, True)]
 IDS = [f"{str(p)[6:]}-{str(g)[6:]}{'-master' if w else ''}" for p, g, w in KINDS]
-SIZES = [1, 3, 16, 31, 32, 33, 255, 1000, 4095, 4096, 4097, 8192 + 17, 20000]
+# the first list has tensors of several blocks, in the others a block takes each tensor whole
+SIZES = {"several": [1, 3, 16, 31, 32, 33, 255, 1000, 4095, 4096, 4097, 8192 + 17, 20000],
+         "whole": [1, 31, 32, 33, 1000, 2048, 2049, 4096, 5000, 8191, 8192], "one": [1000], "least": [8193]}
 HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
 
 
@@ -104,10 +106,11 @@ def check_weights(s, w64, dw, p_dtype):
 # ---------------------------------------------------------------- 32 bits
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
 @pytest.mark.parametrize("offset", [0, 1])
-def test_step_against_64_bits(kind, offset):
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES)
+def test_step_against_64_bits(kind, offset, sizes):
     p_dtype, g_dtype, master = kind
-    states = random_state(SIZES, p_dtype, g_dtype, master, offset, 1)
-    start = [0.0 if i % 2 else 137.0 for i in range(len(SIZES))]
+    states = random_state(sizes, p_dtype, g_dtype, master, offset, 1)
+    start = [0.0 if i % 2 else 137.0 for i in range(len(sizes))]
     steps = torch.tensor(start, device=DEV)
     for k in range(1, 4):
         before = [{x: s[x].t.clone().cpu() for x in "gmv"} | {"w": (s["w"] or s["p"]).t.clone().cpu()} for s in states]
@@ -276,15 +279,16 @@ def check_codes(got, got_scales, x, dx, u, moment):
 
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
 @pytest.mark.parametrize("offset", [0, 1])
-def test_step8_against_64_bits(kind, offset):
+@pytest.mark.parametrize("sizes", SIZES.values(), ids=SIZES)
+def test_step8_against_64_bits(kind, offset, sizes):
     p_dtype, g_dtype, master = kind
-    states = random_state(SIZES, p_dtype, g_dtype, master, offset, 2)
+    states = random_state(sizes, p_dtype, g_dtype, master, offset, 2)
     for s in states:
         encode_state(s)
-    start = [0.0 if i % 2 else 137.0 for i in range(len(SIZES))]
+    start = [0.0 if i % 2 else 137.0 for i in range(len(sizes))]
     steps = torch.tensor(start, device=DEV)
     scale = torch.tensor(0.75, device=DEV)
-    seeds = [i * 1000003 + 5 for i in range(len(SIZES))]
+    seeds = [i * 1000003 + 5 for i in range(len(sizes))]
     for k in range(1, 4):
         before = [{x: s[x].t.clone().cpu() for x in ("g", "m", "v", "ms", "vs")} | {"w": (s["w"] or s["p"]).t.clone().cpu()}
                   for s in states]
