@@ -369,8 +369,14 @@ struct Staged {
   }
 };
 
+// Resident blocks per SM that registers are kept down for, as many as shared memory has room for.
+template <typename W, typename G>
+constexpr int resident8() {
+  return sizeof(W) + sizeof(G) == 4 ? 7 : sizeof(W) + sizeof(G) == 6 ? 6 : 5;
+}
+
 template <typename P, typename G, bool kMaster, int N>
-__global__ void __launch_bounds__(kThreads, 6) adamw8_kernel(const __grid_constant__ Table<N> tab) {
+__global__ void __launch_bounds__(kThreads, resident8<std::conditional_t<kMaster, float, P>, G>()) adamw8_kernel(const __grid_constant__ Table<N> tab) {
   using W = std::conditional_t<kMaster, float, P>;  // what the weights are read from
   struct Stage {
     Staged<uint8_t> m, v;
@@ -545,8 +551,9 @@ __global__ void __launch_bounds__(kThreads, 6) adamw8_kernel(const __grid_consta
           unpack2(mul2(pack2(y0, y1), up), y0, y1);
           asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(half[q]) : "f"(y1), "f"(y0));
           unpack2(mul2(pack2(v[j], v[j + 1]), ve), y0, y1);
-          c[2 * q] = (__float_as_uint(y0) + state8::random_v(h0)) << 4;
-          c[2 * q + 1] = (__float_as_uint(y1) + state8::random_v(h1)) << 4;
+          // (bits + random) << 4; the four bits more of the hash lie below all others and carry nothing
+          c[2 * q] = (__float_as_uint(y0) << 4) + (h0 >> 8);
+          c[2 * q + 1] = (__float_as_uint(y1) << 4) + (h1 >> 8);
         }
         reinterpret_cast<uint32_t*>(mq)[k] = (uint32_t)half[0] | (uint32_t)half[1] << 16;
         const uint32_t vw = __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
@@ -663,18 +670,33 @@ struct Range {
 
 // Refuses a call whose written memory overlaps anything else of the call: two threads would race.
 // `runs`: where each list of tensors begins in r.  Lists are mostly in the order of their addresses
-// already, and merging sorted lists is several times cheaper than sorting.
+// already.  Where they also lie apart from one another neighbours are all there is to compare, else
+// the sorted lists are merged.
 int check_ranges(std::vector<Range>& r, const std::vector<size_t>& runs) {
+  const auto overlap = [] { return fail(FM_ERR_INVALID, "tensors of the step overlap (the same parameter twice?)"); };
   const auto less = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+  std::vector<Range> hulls;
+  hulls.reserve(runs.size());
   for (size_t i = 0; i < runs.size(); ++i) {
-    const auto from = r.begin() + runs[i], to = i + 1 < runs.size() ? r.begin() + runs[i + 1] : r.end();
-    if (!std::is_sorted(from, to, less)) std::sort(from, to, less);
-    std::inplace_merge(r.begin(), from, to, less);
+    const size_t from = runs[i], to = i + 1 < runs.size() ? runs[i + 1] : r.size();
+    if (from == to) continue;
+    if (!std::is_sorted(r.begin() + from, r.begin() + to, less)) std::sort(r.begin() + from, r.begin() + to, less);
+    Range hull = r[from];
+    for (size_t k = from + 1; k < to; ++k) {
+      if (hull.written && r[k].begin < hull.end) return overlap();
+      hull.end = std::max(hull.end, r[k].end);
+    }
+    hulls.push_back(hull);
   }
+  std::sort(hulls.begin(), hulls.end(), less);
+  bool apart = true;
+  for (size_t i = 1; i < hulls.size(); ++i) apart = apart && hulls[i - 1].end <= hulls[i].begin;
+  if (apart) return FM_OK;
+  for (size_t i = 1; i < runs.size(); ++i)
+    std::inplace_merge(r.begin(), r.begin() + runs[i], i + 1 < runs.size() ? r.begin() + runs[i + 1] : r.end(), less);
   uintptr_t any = 0, written = 0;
   for (const Range& x : r) {
-    if (x.begin < (x.written ? any : written))
-      return fail(FM_ERR_INVALID, "tensors of the step overlap (the same parameter twice?)");
+    if (x.begin < (x.written ? any : written)) return overlap();
     any = std::max(any, x.end);
     if (x.written) written = std::max(written, x.end);
   }
