@@ -159,23 +159,24 @@ def test_scale_lr_tensor_and_steps_list():
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("bits", [32, 8])
-def test_a_factor_that_is_not_finite_takes_no_step(bad, bits):
-    p, g = torch.randn(5000, device=DEV), torch.randn(5000, device=DEV)
+@pytest.mark.parametrize("n", [5000, 70000])
+def test_a_factor_that_is_not_finite_takes_no_step(bad, bits, n):
+    p, g = torch.randn(n, device=DEV), torch.randn(n, device=DEV)
     steps = torch.tensor([4.0], device=DEV)
     scale = torch.tensor(bad, device=DEV)
     if bits == 32:
-        st = [torch.randn(5000, device=DEV), torch.rand(5000, device=DEV)]
+        st = [torch.randn(n, device=DEV), torch.rand(n, device=DEV)]
         call = lambda: fm.adamw_step([p], [g], [st[0]], [st[1]], steps, lr=0.1, grad_scale=scale)  # noqa: E731
     else:
-        st = [*fm.adamw8_encode(torch.randn(5000, device=DEV), moment=1), *fm.adamw8_encode(torch.rand(5000, device=DEV), moment=2)]
+        st = [*fm.adamw8_encode(torch.randn(n, device=DEV), moment=1), *fm.adamw8_encode(torch.rand(n, device=DEV), moment=2)]
         call = lambda: fm.adamw8_step([p], [g], *[[x] for x in st], steps, lr=0.1, grad_scale=scale)  # noqa: E731
     before = [x.clone() for x in (p, g, steps, *st)]
     call()
     assert all(torch.equal(a, b) for a, b in zip(before, (p, g, steps, *st)))
 
 
-def test_nan_and_inf_gradients_stay_where_they_are():
-    n = 4200
+@pytest.mark.parametrize("n", [4200, 12000])
+def test_nan_and_inf_gradients_stay_where_they_are(n):
     p, g = torch.randn(n, device=DEV), torch.randn(n, device=DEV)
     g[7], g[4100] = math.nan, math.inf
     m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
@@ -187,15 +188,16 @@ def test_nan_and_inf_gradients_stay_where_they_are():
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-def test_more_tensors_than_a_table_and_empty_ones(bits):
-    """1000 tensors, empty ones among them, equal one call per tensor bit for bit."""
+@pytest.mark.parametrize("count, largest", [(24, 9000), (25, 9000), (96, 9000), (97, 100), (360, 9000), (361, 100), (1000, 9000)])
+def test_tables_of_all_lengths_and_empty_tensors(bits, count, largest):
+    """Up to 1000 tensors, empty ones among them, equal one call per tensor bit for bit."""
     r = gen(5)
-    sizes = [(i * 37) % 131 if i % 10 else 0 for i in range(1000)]
-    sizes[500] = 9000
+    sizes = [(i * 37) % 131 if i % 10 else 0 for i in range(count)]
+    sizes[count // 2] = largest
     p = [torch.randn(n, device=DEV, generator=r) for n in sizes]
     g = [torch.randn(n, device=DEV, generator=r) for n in sizes]
     q = [x.clone() for x in p]
-    steps, again = torch.zeros(1000, device=DEV), torch.zeros(1000, device=DEV)
+    steps, again = torch.zeros(count, device=DEV), torch.zeros(count, device=DEV)
 
     def states():
         if bits == 32:
@@ -206,12 +208,31 @@ def test_more_tensors_than_a_table_and_empty_ones(bits):
     a, b = states(), states()
     for _ in range(2):
         step(p, g, *a, steps, lr=0.1, **({} if bits == 32 else {"seeds": 50}))
-        for i in range(1000):
+        for i in range(count):
             step([q[i]], [g[i]], *[[x[i]] for x in b], again[i:i + 1], lr=0.1, **({} if bits == 32 else {"seeds": [50 + i]}))
     assert (steps == 2).all() and (again == 2).all()
     assert all(torch.equal(x, y) for x, y in zip(p, q))
     for xs, ys in zip(a, b):
         assert all(torch.equal(x, y) for x, y in zip(xs, ys))
+
+
+@pytest.mark.parametrize("n", [500, 9000])
+def test_many_groups_of_one_kind(n):
+    """More groups than one launch holds, each with its own settings."""
+    make = lambda: [torch.nn.Parameter(torch.linspace(-1, 1, n, device=DEV)) for _ in range(20)]  # noqa: E731
+    ps, qs = make(), make()
+    a = fm.AdamW([dict(params=[p], lr=0.01 * (i + 1), betas=(0.5 + 0.02 * i, 0.9), eps=1e-8 * (i + 1), weight_decay=0.05 * i)
+                  for i, p in enumerate(ps)])
+    b = [fm.AdamW([q], **{k: g[k] for k in ("lr", "betas", "eps", "weight_decay")}) for q, g in zip(qs, a.param_groups)]
+    for p, q in zip(ps, qs):
+        p.grad = torch.randn(n, device=DEV)
+        q.grad = p.grad.clone()
+    for _ in range(2):
+        a.step()
+        for opt in b:
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    assert len({float(p.detach()[0]) for p in ps}) == 20
 
 
 def test_groups_of_all_kinds_in_one_call():
