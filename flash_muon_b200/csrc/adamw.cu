@@ -864,7 +864,9 @@ struct Batch {
     if (last_group != gi) {
       Hyper& h = tab.h[hypers++];
       h.lr = g.lr; h.beta1 = g.beta1; h.beta2 = g.beta2; h.lr_dev = g.lr_device;
-      h.wd = g.weight_decay; h.eps = (float)g.eps;
+      h.wd = g.weight_decay;
+      // the smallest stored second moment is 2^-126; a step may leave less, whose approximate root is 0
+      h.eps = g.state_bits == 8 ? std::max((float)g.eps, 0x1p-64f) : (float)g.eps;
       h.b1 = (float)g.beta1; h.omb1 = (float)(1.0 - g.beta1);
       h.b2 = (float)g.beta2; h.omb2 = (float)(1.0 - g.beta2);
       last_group = gi;

@@ -273,6 +273,8 @@ int fm_muon_step(const fm_muon_group* groups, int ngroups, void* const* workspac
  * chance of the distance; the random numbers are a function of seeds[i], the step count and the
  * element's index, so equal calls give equal bits.  A value that is not finite becomes "not a
  * number" (first moment, code 127) or infinity (second, code 255) and leaves its neighbours alone.
+ * Scales are at least 17 (first moment) and 32 (second); a positive second moment is never stored
+ * as zero; eps below 2^-64 counts as 2^-64.
  */
 typedef struct {
   void* const* params;

@@ -374,6 +374,23 @@ def test_step8_values_that_are_not_finite():
     assert p[near].isfinite().all()
 
 
+def test_step8_without_eps():
+    """Gradients whose squares are subnormal, or zero: no division by zero although eps is zero."""
+    n = 3000
+    g = torch.zeros(n, device=DEV)
+    for i, x in enumerate((1e-25, 1e-21, 1e-19, 1e-17, 1e-12, 1.0)):
+        g[i * 320 + 5:(i + 1) * 320] = x
+    p = torch.zeros(n, device=DEV)
+    st = [[torch.zeros(-(-n // 32) * k, dtype=torch.uint8, device=DEV)] for k in (32, 1, 32, 1)]
+    steps = torch.zeros(1, device=DEV)
+    for _ in range(3):
+        fm.adamw8_step([p], [g], *st, steps, lr=1.0, weight_decay=0.0, eps=0.0)
+        assert p.isfinite().all() and (p[g == 0] == 0).all()
+        g.mul_(0.5)
+    # where the squares are normal numbers a first step is lr, later ones with shrinking gradients less than 2
+    assert (p[g > 1e-18].abs() <= 5.0).all() and (p[g > 1e-18].abs() >= 1.0).all()
+
+
 def test_step8_is_right_on_average():
     """The mean over 4096 seeds of the stored moments is the moment: rounding is unbiased.  A code's
     step is at most 1/8 of the value, so the mean of N values has a standard deviation of at most
