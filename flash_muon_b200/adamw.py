@@ -147,7 +147,9 @@ class AdamW(torch.optim.Optimizer):
     ``betas``, ``eps`` and ``weight_decay`` as in ``torch.optim.AdamW``.  ``state_bits`` 8 keeps the
     moments in 8 bits for parameters of at least ``min_8bit_numel`` elements (10.1 instead of 22 bytes
     of traffic per bfloat16 element and step, 2.06 instead of 8 bytes of state); ``master_weights``
-    keeps a float32 copy of 16-bit parameters.  Every setting can differ between parameter groups.
+    keeps a float32 copy of 16-bit parameters, made at the first step, from which the parameter is
+    written: weights that are loaded later need ``state[p]["master"]`` written too.  Every setting can
+    differ between parameter groups.
 
     State per parameter: ``step`` (float32 scalar on the device), ``exp_avg`` and ``exp_avg_sq``
     (float32 in the parameter's shape, or flat uint8 with ``exp_avg_scale`` and ``exp_avg_sq_scale``),
@@ -196,7 +198,6 @@ class AdamW(torch.optim.Optimizer):
             state["master"] = p.detach().float().contiguous().clone()
         return state
 
-    @torch.no_grad()
     def step(self, closure=None, *, grad_scale: Tensor | None = None):
         """One step of every parameter that has a gradient.  ``grad_scale``: see ``adamw_step``."""
         loss = None

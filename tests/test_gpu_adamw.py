@@ -351,6 +351,16 @@ def test_values_and_encode(moment, dtype, n):
         assert vals.dtype == out and torch.equal(vals.double().cpu(), A.decode(codes, scales, moment)[:n])
 
 
+@pytest.mark.parametrize("offset", [0, 3, 32])
+def test_values_of_states_at_any_address(offset):
+    n = 5 * 4096 + 32
+    codes, scales = fm.adamw8_encode(torch.randn(n, device=DEV, generator=gen(1)), moment=1)
+    moved = Guarded(codes, offset)
+    for dtype in (F32, B16, H16):
+        assert torch.equal(fm.adamw8_values(moved.t, scales, moment=1, dtype=dtype),
+                           fm.adamw8_values(codes, scales, moment=1, dtype=F32).to(dtype))
+
+
 def test_step8_values_that_are_not_finite():
     """An element that is not finite costs neither its neighbours nor the block's scale."""
     n = 96
@@ -501,6 +511,36 @@ def test_capture_without_state_is_refused():
             opt.step()
     opt.step()
     assert float(opt.state[p]["step"]) == 1.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_optimizers_on_two_streams_at_once(bits):
+    def make(seed):
+        torch.manual_seed(seed)
+        ps = [torch.nn.Parameter(torch.randn(n, device=DEV).to(B16)) for n in (2_000_000, 5000, 33)]
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        return ps, fm.AdamW(ps, state_bits=bits, seed=seed)
+
+    def go(ps, opt):
+        for _ in range(10):
+            _, scale = fm.grad_norm([p.grad for p in ps], 1.0)
+            opt.step(grad_scale=scale)
+
+    apart = [make(1), make(2)]
+    for x in apart:
+        go(*x)
+    together = [make(1), make(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for stream, (ps, opt) in zip(streams, together):
+            with torch.cuda.stream(stream):
+                _, scale = fm.grad_norm([p.grad for p in ps], 1.0)
+                opt.step(grad_scale=scale)
+    torch.cuda.synchronize()
+    for (ps, _), (qs, _) in zip(apart, together):
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
 
 
 def test_step_waits_for_the_gradients_of_its_stream():
