@@ -204,45 +204,16 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        by_device: dict[int, list[tuple]] = {}
-        index = 0
-        for group in self.param_groups:
-            kinds: dict[tuple, tuple] = {}
-            for p in group["params"]:
-                index += 1
-                grad = p.grad
-                if grad is None:
-                    continue
-                state = self.state.get(p)
-                if not state:
-                    assert p.is_cuda, "`params` must be CUDA tensors"
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("take one step before capturing: a parameter has no state yet")
-                    state = self._init_state(p, group)
-                eight, master = "exp_avg_scale" in state, state.get("master")
-                kind = (p.get_device(), eight, master is not None)
-                lists = kinds.get(kind)
-                if lists is None:  # params, grads, masters, moments, scales, steps, seeds
-                    lists = kinds[kind] = ([], [], None if master is None else [], [], [], [] if eight else None,
-                                           [] if eight else None, [], [] if eight else None)
-                lists[0].append(p)
-                lists[1].append(grad)
-                lists[3].append(state["exp_avg"])
-                lists[4].append(state["exp_avg_sq"])
-                lists[7].append(state["step"])
-                if master is not None:
-                    lists[2].append(master)
-                if eight:
-                    lists[5].append(state["exp_avg_scale"])
-                    lists[6].append(state["exp_avg_sq_scale"])
-                    lists[8].append(group["seed"] + index)
-            for kind, lists in kinds.items():
-                by_device.setdefault(kind[0], []).append(
-                    (*lists, group["lr"], *group["betas"], group["eps"], group["weight_decay"]))
-        for groups in by_device.values():
-            rc = _host.adamw_step(_STEP, groups, grad_scale)
-            if rc:
-                check(rc)
+        rc = _host.optimizer_step(_STEP, self.param_groups, self.state, grad_scale)
+        if isinstance(rc, list):  # parameters that have no state yet
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("take one step before capturing: a parameter has no state yet")
+            for p, group in rc:
+                with torch.cuda.device(p.device):
+                    self._init_state(p, group)
+            rc = _host.optimizer_step(_STEP, self.param_groups, self.state, grad_scale)
+        if rc:
+            check(rc)
         return loss
 
     def state_values(self, p: Tensor) -> tuple[Tensor, Tensor]:

@@ -768,6 +768,10 @@ int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges, std
   }
   runs.push_back(ranges.size());
   for (int i = 0; i < g.count; ++i) ranges.push_back({(uintptr_t)g.steps[i], (uintptr_t)g.steps[i] + 4, true});
+  if (g.lr_device) {
+    runs.push_back(ranges.size());
+    ranges.push_back({(uintptr_t)g.lr_device, (uintptr_t)g.lr_device + 4, false});
+  }
   return FM_OK;
 }
 
@@ -898,7 +902,7 @@ struct Batch {
 };
 
 // Parts of a tile with 8-bit states: what a block spends on its tensor's coefficients is shared by up to
-// 8 of them once that leaves every SM two rounds of blocks (8 are resident).
+// 8 of them, as many as leave every SM 12 blocks (5 to 7 are resident).
 int parts_of(long long elements) {
   const long long parts = elements / ((long long)kPart8 * 12 * sm_count() + 1);
   return parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : (int)parts;
@@ -927,15 +931,19 @@ int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cu
   std::vector<Range> ranges;
   size_t tensors = 0;
   for (int gi = 0; gi < ngroups; ++gi) tensors += groups[gi].count > 0 ? groups[gi].count : 0;
-  ranges.reserve(tensors * 8);
+  ranges.reserve(tensors * 8 + ngroups + 1);
   std::vector<size_t> runs;
-  runs.reserve(ngroups * 8);
+  runs.reserve(ngroups * 9 + 1);
   for (int gi = 0; gi < ngroups; ++gi) {
     const int rc = check_group(groups[gi], gi, ranges, runs);
     if (rc != FM_OK) return rc;
   }
   if (tensors == 0) return FM_OK;
   if (!aligned(scale, 4)) return fail(FM_ERR_INVALID, "misaligned gradient scale");
+  if (scale) {
+    runs.push_back(ranges.size());
+    ranges.push_back({(uintptr_t)scale, (uintptr_t)scale + 4, false});
+  }
   int rc = check_ranges(ranges, runs);
   if (rc != FM_OK) return rc;
 

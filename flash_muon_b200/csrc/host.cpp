@@ -1,6 +1,6 @@
 // Python side of the multi-tensor entry points: checks lists of tensors and turns them into the C
 // ABI's arrays.  A call over 65 tensors and four lists makes 1500 attribute look-ups, 100 us in
-// Python against 6 us on the GPU; here they take 3 us.
+// Python against 6 us on the GPU; here they take 4 us.
 // The C entries are given by address, so this module is bound to no particular shared library.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -89,33 +89,6 @@ double number(PyObject* o) {
   return x;
 }
 
-// Addresses of a list of tensors that go with the parameters: checked for place and, where given, for
-// type and size (`per` elements of the parameter, rounded up to blocks of 32, per element here).
-std::vector<void*> addresses(PyObject* list, const char* name, int device, const std::vector<int64_t>& numels,
-                             std::optional<at::ScalarType> dtype, int per = 0) {
-  const Items items(list, name);
-  REQUIRE(items.size() == (Py_ssize_t)numels.size(), "lists must have one entry per parameter");
-  std::vector<void*> out;
-  out.reserve(numels.size());
-  for (Py_ssize_t i = 0; i < items.size(); ++i) {
-    const at::Tensor& t = tensor(items[i], name);
-    check_place(t, name, device);
-    if (per == 0) {
-      REQUIRE(t.numel() == numels[i], "`%s` must have the parameters' sizes", name);
-    }
-    if (dtype) {
-      REQUIRE(t.scalar_type() == *dtype, "`%s` must be torch.%s", name, *dtype == at::kFloat ? "float32" : "uint8");
-    }
-    if (per != 0) {
-      const int64_t blocks = (numels[i] + 31) / 32;
-      REQUIRE(t.numel() == (per == 1 ? blocks * 32 : blocks), "`%s` must have one byte per %s", name,
-              per == 1 ? "element, padded to 32" : "block of 32");
-    }
-    out.push_back(t.data_ptr());
-  }
-  return out;
-}
-
 // One parameter group of a call, in arrays that live until the call returns.
 struct Group {
   std::vector<int64_t> numels;
@@ -124,120 +97,164 @@ struct Group {
   fm_adamw_group g;
 };
 
+// What a parameter is stepped with; master, scales may be null.
+struct Row {
+  const at::Tensor *p, *grad, *master, *m, *v, *ms, *vs;
+  void* step;
+  uint32_t seed;
+};
+
+void* step_count(const at::Tensor& t, int device) {
+  check_place(t, "steps", device);
+  REQUIRE(t.scalar_type() == at::kFloat, "`steps` must be torch.float32");
+  REQUIRE(t.numel() == 1, "`steps` must be scalars");
+  return t.data_ptr();
+}
+
+// Takes the rows of one parameter group, checks them and sorts them by kind (types, masters, state bits).
+class Builder {
+ public:
+  Builder(std::vector<Group>& out, int device, const fm_adamw_group& settings)
+      : out_(out), first_(out.size()), device_(device), settings_(settings) {
+    const fm_adamw_group& g = settings;
+    REQUIRE(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0, "betas must lie in [0, 1)");
+    REQUIRE(g.eps >= 0.0 && std::isfinite(g.eps), "eps must be finite and not negative");
+    REQUIRE(std::isfinite(g.lr) && std::isfinite(g.weight_decay), "lr and weight_decay must be finite");
+  }
+
+  void add(const Row& r, size_t expected) {
+    check_place(*r.p, "params", device_);
+    check_place(*r.grad, "grads", device_);
+    const int64_t n = r.p->numel(), blocks = (n + 31) / 32;
+    REQUIRE(r.grad->numel() == n, "`grads` must have the parameters' sizes");
+    const int pd = dtype_code(r.p->scalar_type()), gd = dtype_code(r.grad->scalar_type());
+    const bool eight = r.ms != nullptr;
+    moment(*r.m, "exp_avgs", eight, n, blocks);
+    moment(*r.v, "exp_avg_sqs", eight, n, blocks);
+    if (eight) {
+      scales(*r.ms, "exp_avg_scales", blocks);
+      scales(*r.vs, "exp_avg_sq_scales", blocks);
+    }
+    if (r.master) {
+      check_place(*r.master, "masters", device_);
+      REQUIRE(r.master->numel() == n, "`masters` must have the parameters' sizes");
+      REQUIRE(r.master->scalar_type() == at::kFloat, "`masters` must be torch.float32");
+      REQUIRE(pd != FM_F32, "float32 parameters have no master copies");
+    }
+    Group& x = group(pd, gd, eight, r.master != nullptr, expected);
+    x.numels.push_back(n);
+    x.params.push_back(r.p->data_ptr());
+    x.grads.push_back(r.grad->data_ptr());
+    x.m.push_back(r.m->data_ptr());
+    x.v.push_back(r.v->data_ptr());
+    x.steps.push_back(r.step);
+    if (r.master) x.masters.push_back(r.master->data_ptr());
+    if (eight) {
+      x.ms.push_back(r.ms->data_ptr());
+      x.vs.push_back(r.vs->data_ptr());
+      x.seeds.push_back(r.seed);
+    }
+  }
+
+ private:
+  void moment(const at::Tensor& t, const char* name, bool eight, int64_t n, int64_t blocks) {
+    check_place(t, name, device_);
+    REQUIRE(t.scalar_type() == (eight ? at::kByte : at::kFloat), "`%s` must be torch.%s", name, eight ? "uint8" : "float32");
+    if (eight) REQUIRE(t.numel() == blocks * 32, "`%s` must have one byte per element, padded to 32", name);
+    else REQUIRE(t.numel() == n, "`%s` must have the parameters' sizes", name);
+  }
+  void scales(const at::Tensor& t, const char* name, int64_t blocks) {
+    check_place(t, name, device_);
+    REQUIRE(t.scalar_type() == at::kByte, "`%s` must be torch.uint8", name);
+    REQUIRE(t.numel() == blocks, "`%s` must have one byte per block of 32", name);
+  }
+  Group& group(int pd, int gd, bool eight, bool master, size_t expected) {
+    for (size_t i = first_; i < out_.size(); ++i) {
+      Group& x = out_[i];
+      if (x.g.p_dtype == pd && x.g.g_dtype == gd && (x.g.state_bits == 8) == eight && !x.masters.empty() == master) return x;
+    }
+    out_.emplace_back();
+    Group& x = out_.back();
+    x.g = settings_;
+    x.g.p_dtype = pd;
+    x.g.g_dtype = gd;
+    x.g.state_bits = eight ? 8 : 32;
+    for (std::vector<void*>* v : {&x.params, &x.grads, &x.m, &x.v, &x.steps}) v->reserve(expected);
+    x.numels.reserve(expected);
+    if (master) x.masters.reserve(expected);
+    if (eight) {
+      x.ms.reserve(expected);
+      x.vs.reserve(expected);
+      x.seeds.reserve(expected);
+    }
+    return x;
+  }
+
+  std::vector<Group>& out_;
+  const size_t first_;
+  const int device_;
+  const fm_adamw_group settings_;
+};
+
+void learning_rate(PyObject* lr, int device, fm_adamw_group& g) {
+  if (THPVariable_Check(lr)) g.lr_device = static_cast<const float*>(scalar(lr, "lr", device));
+  else g.lr = number(lr);
+}
+
+uint32_t seed_of(PyObject* o) {
+  const uint32_t s = (uint32_t)PyLong_AsUnsignedLongLongMask(o);
+  if (PyErr_Occurred()) throw Refused{};
+  return s;
+}
+
 // (params, grads, masters, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, steps, seeds, lr, beta1,
-// beta2, eps, weight_decay); masters, scales and seeds may be None.  Appends one group per pair of types.
+// beta2, eps, weight_decay); masters, scales and seeds may be None.
 void parse_group(PyObject* tuple, int& device, std::vector<Group>& out) {
   const Items f(tuple, "group");
   REQUIRE(f.size() == 14, "a group has 14 entries");
   const Items params(f[0], "params"), grads(f[1], "grads");
-  const size_t n = params.size();
+  const Py_ssize_t n = params.size();
   if (n == 0) return;
-  REQUIRE((size_t)grads.size() == n, "lists must have one entry per parameter");
-  std::vector<int64_t> numels(n);
-  std::vector<uint8_t> kinds(n);  // pair of types
-  std::vector<void*> ps(n), gs(n);
-  bool one_kind = true, any_f32 = false;
-  for (size_t i = 0; i < n; ++i) {
-    const at::Tensor &p = tensor(params[i], "params"), &g = tensor(grads[i], "grads");
-    if (device < 0 && p.is_cuda()) device = p.get_device();
-    check_place(p, "params", device);
-    check_place(g, "grads", device);
-    REQUIRE(g.numel() == p.numel(), "`grads` must have the parameters' sizes");
-    numels[i] = p.numel();
-    const int pd = dtype_code(p.scalar_type());
-    kinds[i] = (uint8_t)(pd * 4 + dtype_code(g.scalar_type()));
-    one_kind = one_kind && kinds[i] == kinds[0];
-    any_f32 = any_f32 || pd == FM_F32;
-    ps[i] = p.data_ptr();
-    gs[i] = g.data_ptr();
-  }
-  const bool eight = f[5] != Py_None;
-  const auto state = eight ? at::kByte : at::kFloat;
-  const int per = eight ? 1 : 0;
-  std::vector<void*> m = addresses(f[3], "exp_avgs", device, numels, state, per);
-  std::vector<void*> v = addresses(f[4], "exp_avg_sqs", device, numels, state, per);
-  std::vector<void*> w, ms, vs;
-  if (f[2] != Py_None) {
-    w = addresses(f[2], "masters", device, numels, at::kFloat);
-    REQUIRE(!any_f32, "float32 parameters have no master copies");
-  }
-  std::vector<uint32_t> seeds;
-  if (eight) {
-    ms = addresses(f[5], "exp_avg_scales", device, numels, at::kByte, 32);
-    vs = addresses(f[6], "exp_avg_sq_scales", device, numels, at::kByte, 32);
-    const Items s(f[8], "seeds");
-    REQUIRE((size_t)s.size() == n, "lists must have one entry per parameter");
-    seeds.resize(n);
-    for (size_t i = 0; i < n; ++i) {
-      seeds[i] = (uint32_t)PyLong_AsUnsignedLongLongMask(s[i]);
-      if (PyErr_Occurred()) throw Refused{};
-    }
-  }
-  std::vector<void*> steps(n);
-  if (THPVariable_Check(f[7])) {
+  const bool eight = f[5] != Py_None, master = f[2] != Py_None;
+  const Items m(f[3], "exp_avgs"), v(f[4], "exp_avg_sqs");
+  std::optional<Items> w, ms, vs, seeds, steps;
+  auto list = [&](std::optional<Items>& items, int k, const char* name) {
+    items.emplace(f[k], name);
+    return items->size() == n;
+  };
+  bool same = grads.size() == n && m.size() == n && v.size() == n;
+  if (master) same = list(w, 2, "masters") && same;
+  if (eight) same = list(ms, 5, "exp_avg_scales") && list(vs, 6, "exp_avg_sq_scales") && list(seeds, 8, "seeds") && same;
+  float* counts = nullptr;
+  if (!THPVariable_Check(f[7])) same = list(steps, 7, "steps") && same;
+  REQUIRE(same, "lists must have one entry per parameter");
+  const at::Tensor& p0 = tensor(params[0], "params");
+  REQUIRE(p0.is_cuda(), "`params` must be CUDA tensors");
+  if (device < 0) device = p0.get_device();
+  if (!steps) {
     const at::Tensor& t = THPVariable_Unpack(f[7]);
-    REQUIRE(t.dim() == 1 && (size_t)t.numel() == n, "`steps` must have one count per parameter");
+    REQUIRE(t.dim() == 1 && t.numel() == n, "`steps` must have one count per parameter");
     check_place(t, "steps", device);
     REQUIRE(t.scalar_type() == at::kFloat, "`steps` must be torch.float32");
-    for (size_t i = 0; i < n; ++i) steps[i] = static_cast<float*>(t.data_ptr()) + i;
-  } else {
-    const Items s(f[7], "steps");
-    REQUIRE((size_t)s.size() == n, "lists must have one entry per parameter");
-    for (size_t i = 0; i < n; ++i) {
-      const at::Tensor& t = tensor(s[i], "steps");
-      check_place(t, "steps", device);
-      REQUIRE(t.scalar_type() == at::kFloat, "`steps` must be torch.float32");
-      REQUIRE(t.numel() == 1, "`steps` must be scalars");
-      steps[i] = t.data_ptr();
-    }
+    counts = static_cast<float*>(t.data_ptr());
   }
   fm_adamw_group g = {};
-  g.state_bits = eight ? 8 : 32;
-  if (THPVariable_Check(f[9]))
-    g.lr_device = static_cast<const float*>(scalar(f[9], "lr", device));
-  else
-    g.lr = number(f[9]);
+  learning_rate(f[9], device, g);
   g.beta1 = number(f[10]);
   g.beta2 = number(f[11]);
   g.eps = number(f[12]);
   g.weight_decay = number(f[13]);
-  REQUIRE(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0, "betas must lie in [0, 1)");
-  REQUIRE(g.eps >= 0.0 && std::isfinite(g.eps), "eps must be finite and not negative");
-  REQUIRE(std::isfinite(g.lr) && std::isfinite(g.weight_decay), "lr and weight_decay must be finite");
-
-  auto add = [&](uint8_t kind, Group&& x) {
-    x.g = g;
-    x.g.p_dtype = kind / 4;
-    x.g.g_dtype = kind % 4;
-    x.g.count = (int32_t)x.numels.size();
-    out.push_back(std::move(x));
-  };
-  if (one_kind) {
-    Group x;
-    x.numels = std::move(numels); x.params = std::move(ps); x.grads = std::move(gs); x.masters = std::move(w);
-    x.m = std::move(m); x.v = std::move(v); x.ms = std::move(ms); x.vs = std::move(vs);
-    x.steps = std::move(steps); x.seeds = std::move(seeds);
-    add(kinds[0], std::move(x));
-    return;
-  }
-  for (int kind = 0; kind < 12; ++kind) {
-    Group x;
-    for (size_t i = 0; i < n; ++i) {
-      if (kinds[i] != kind) continue;
-      x.numels.push_back(numels[i]);
-      x.params.push_back(ps[i]);
-      x.grads.push_back(gs[i]);
-      x.m.push_back(m[i]);
-      x.v.push_back(v[i]);
-      x.steps.push_back(steps[i]);
-      if (!w.empty()) x.masters.push_back(w[i]);
-      if (eight) {
-        x.ms.push_back(ms[i]);
-        x.vs.push_back(vs[i]);
-        x.seeds.push_back(seeds[i]);
-      }
+  Builder rows(out, device, g);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    Row r = {&tensor(params[i], "params"), &tensor(grads[i], "grads"), master ? &tensor((*w)[i], "masters") : nullptr,
+             &tensor(m[i], "exp_avgs"), &tensor(v[i], "exp_avg_sqs"), nullptr, nullptr, nullptr, 0};
+    if (eight) {
+      r.ms = &tensor((*ms)[i], "exp_avg_scales");
+      r.vs = &tensor((*vs)[i], "exp_avg_sq_scales");
+      r.seed = seed_of((*seeds)[i]);
     }
-    if (!x.numels.empty()) add((uint8_t)kind, std::move(x));
+    r.step = steps ? step_count(tensor((*steps)[i], "steps"), device) : counts + i;
+    rows.add(r, n);
   }
 }
 
@@ -270,6 +287,30 @@ void need(Py_ssize_t have, Py_ssize_t want) {
   throw Refused{};
 }
 
+int launch(decltype(&fm_adamw_step) fn, std::vector<Group>& groups, int device, PyObject* grad_scale) {
+  if (groups.empty()) return FM_OK;
+  const float* scale = grad_scale == Py_None ? nullptr : static_cast<const float*>(scalar(grad_scale, "grad_scale", device));
+  std::vector<fm_adamw_group> table;
+  table.reserve(groups.size());
+  for (Group& x : groups) {
+    auto at = [](std::vector<void*>& p) { return p.empty() ? nullptr : p.data(); };
+    x.g.params = at(x.params);
+    x.g.grads = at(x.grads);
+    x.g.masters = at(x.masters);
+    x.g.exp_avg = at(x.m);
+    x.g.exp_avg_sq = at(x.v);
+    x.g.exp_avg_scale = at(x.ms);
+    x.g.exp_avg_sq_scale = at(x.vs);
+    x.g.steps = reinterpret_cast<float* const*>(at(x.steps));
+    x.g.numels = x.numels.data();
+    x.g.seeds = x.seeds.empty() ? nullptr : x.seeds.data();
+    x.g.count = (int32_t)x.numels.size();
+    table.push_back(x.g);
+  }
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  return fn(table.data(), (int)table.size(), scale, c10::cuda::getCurrentCUDAStream().stream());
+}
+
 // adamw_step(fm_adamw_step, groups, grad_scale or None) -> status
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -280,26 +321,117 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     groups.reserve(tuples.size() + 4);
     int device = -1;
     for (Py_ssize_t i = 0; i < tuples.size(); ++i) parse_group(tuples[i], device, groups);
-    if (groups.empty()) return PyLong_FromLong(FM_OK);
-    const float* scale = a[2] == Py_None ? nullptr : static_cast<const float*>(scalar(a[2], "grad_scale", device));
-    std::vector<fm_adamw_group> table;
-    table.reserve(groups.size());
-    for (Group& x : groups) {
-      auto at = [](std::vector<void*>& p) { return p.empty() ? nullptr : p.data(); };
-      x.g.params = at(x.params);
-      x.g.grads = at(x.grads);
-      x.g.masters = at(x.masters);
-      x.g.exp_avg = at(x.m);
-      x.g.exp_avg_sq = at(x.v);
-      x.g.exp_avg_scale = at(x.ms);
-      x.g.exp_avg_sq_scale = at(x.vs);
-      x.g.steps = reinterpret_cast<float* const*>(at(x.steps));
-      x.g.numels = x.numels.data();
-      x.g.seeds = x.seeds.empty() ? nullptr : x.seeds.data();
-      table.push_back(x.g);
+    return PyLong_FromLong(launch(fn, groups, device, a[2]));
+  });
+}
+
+// A dictionary's entry (borrowed), or null.
+PyObject* entry_of(PyObject* dict, PyObject* key) {
+  PyObject* x = PyDict_GetItemWithError(dict, key);
+  if (!x && PyErr_Occurred()) throw Refused{};
+  return x;
+}
+
+PyObject* setting(PyObject* dict, const char* name) {
+  PyObject* x = PyDict_GetItemString(dict, name);
+  if (!x) {
+    PyErr_Format(PyExc_KeyError, "parameter group without `%s`", name);
+    throw Refused{};
+  }
+  return x;
+}
+
+// optimizer_step(fm_adamw_step, param_groups, state, grad_scale or None) -> status, or the list of
+// (parameter, group) that have a gradient and no state yet; nothing is launched then.
+PyObject* optimizer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    need(n, 4);
+    const auto fn = entry<decltype(&fm_adamw_step)>(a[0]);
+    static PyObject* const k_m = PyUnicode_InternFromString("exp_avg");
+    static PyObject* const k_v = PyUnicode_InternFromString("exp_avg_sq");
+    static PyObject* const k_ms = PyUnicode_InternFromString("exp_avg_scale");
+    static PyObject* const k_vs = PyUnicode_InternFromString("exp_avg_sq_scale");
+    static PyObject* const k_step = PyUnicode_InternFromString("step");
+    static PyObject* const k_master = PyUnicode_InternFromString("master");
+    REQUIRE(PyDict_Check(a[2]), "`state` must be a dictionary");
+    const Items param_groups(a[1], "param_groups");
+    struct Missing {  // released on every way out
+      PyObject* list = nullptr;
+      ~Missing() { Py_XDECREF(list); }
+    } missing;
+    struct Device {
+      int index;
+      std::vector<Group> groups;
+    };
+    std::vector<Device> devices;
+    int64_t index = 0;
+    for (Py_ssize_t gi = 0; gi < param_groups.size(); ++gi) {
+      PyObject* group = param_groups[gi];
+      REQUIRE(PyDict_Check(group), "parameter groups must be dictionaries");
+      const Items params(setting(group, "params"), "params");
+      const Items betas(setting(group, "betas"), "betas");
+      REQUIRE(betas.size() == 2, "`betas` must be a pair");
+      fm_adamw_group g = {};
+      g.beta1 = number(betas[0]);
+      g.beta2 = number(betas[1]);
+      g.eps = number(setting(group, "eps"));
+      g.weight_decay = number(setting(group, "weight_decay"));
+      PyObject* lr = setting(group, "lr");
+      const uint32_t seed = seed_of(setting(group, "seed"));
+      int builder_device = -1;
+      std::optional<Builder> rows;
+      for (Py_ssize_t i = 0; i < params.size(); ++i) {
+        ++index;
+        const at::Tensor& p = tensor(params[i], "params");
+        const at::Tensor& grad = p.grad();
+        if (!grad.defined()) continue;
+        REQUIRE(p.is_cuda(), "`params` must be CUDA tensors");
+        REQUIRE(grad.layout() == at::kStrided, "AdamW takes no sparse gradients");
+        PyObject* state = entry_of(a[2], params[i]);
+        if (!state || !PyDict_Check(state) || PyDict_GET_SIZE(state) == 0) {
+          if (!missing.list) missing.list = PyList_New(0);
+          PyObject* pair = missing.list ? PyTuple_Pack(2, params[i], group) : nullptr;
+          const bool kept = pair && PyList_Append(missing.list, pair) == 0;
+          Py_XDECREF(pair);
+          if (!kept) throw Refused{};
+          continue;
+        }
+        if (missing.list) continue;
+        const int device = p.get_device();
+        if (device != builder_device) {
+          size_t d = 0;
+          while (d < devices.size() && devices[d].index != device) ++d;
+          if (d == devices.size()) {
+            devices.push_back({device, {}});
+            devices.back().groups.reserve(param_groups.size() * 2 + 4);
+          }
+          learning_rate(lr, device, g);
+          rows.emplace(devices[d].groups, device, g);
+          builder_device = device;
+        }
+        auto get = [&](PyObject* key, const char* name, bool needed) -> const at::Tensor* {
+          PyObject* x = entry_of(state, key);
+          REQUIRE(x || !needed, "state of a parameter without `%s`", name);
+          return x ? &tensor(x, name) : nullptr;
+        };
+        Row r = {&p, &grad, get(k_master, "masters", false), get(k_m, "exp_avgs", true), get(k_v, "exp_avg_sqs", true),
+                 get(k_ms, "exp_avg_scales", false), nullptr, nullptr, (uint32_t)(seed + (uint32_t)index)};
+        if (r.ms) r.vs = get(k_vs, "exp_avg_sq_scales", true);
+        r.step = step_count(*get(k_step, "steps", true), device);
+        rows->add(r, params.size());
+      }
     }
-    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
-    return PyLong_FromLong(fn(table.data(), (int)table.size(), scale, c10::cuda::getCurrentCUDAStream().stream()));
+    if (missing.list) {
+      PyObject* list = missing.list;
+      missing.list = nullptr;
+      return list;
+    }
+    int rc = FM_OK;
+    for (Device& d : devices) {
+      rc = launch(fn, d.groups, d.index, a[3]);
+      if (rc != FM_OK) break;
+    }
+    return PyLong_FromLong(rc);
   });
 }
 
@@ -393,6 +525,7 @@ PyObject* adamw8_values(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw_step)), METH_FASTCALL, nullptr},
+    {"optimizer_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(optimizer_step)), METH_FASTCALL, nullptr},
     {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_norm)), METH_FASTCALL, nullptr},
     {"scale", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scale)), METH_FASTCALL, nullptr},
     {"adamw8_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw8_values)), METH_FASTCALL, nullptr},

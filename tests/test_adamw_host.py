@@ -136,6 +136,8 @@ def test_step_refuses_bad_group_lists_and_scale():
     assert lib.fm_adamw_step(None, 0, None, None) == 0
     assert Call(count=0)() == 0
     assert Call()(0x90002) == INVALID and b"gradient scale" in lib.fm_last_error()
+    assert Call()(0x10000 + 8) == INVALID and b"overlap" in lib.fm_last_error()          # inside the parameter
+    assert Call(lr_device=0x80000)() == INVALID and b"overlap" in lib.fm_last_error()    # the count itself
 
 
 def test_struct_layout_is_the_header_s():
