@@ -126,7 +126,8 @@ def grad_norm(grads: Sequence[Tensor], max_norm: float = math.inf) -> tuple[Tens
 def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float) -> Tensor:
     """Scales the gradients of ``parameters`` in place so that their norm is at most ``max_norm`` and
     returns the norm they had (``torch.nn.utils.clip_grad_norm_`` for the Euclidean norm).  Gradients
-    within the norm are read once and left alone; if the norm is not finite all become NaN."""
+    within the norm are read once and left alone; if the norm is not finite all become NaN.  A parameter
+    that is given twice is refused."""
     if isinstance(parameters, Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]

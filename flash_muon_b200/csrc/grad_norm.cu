@@ -4,8 +4,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
+#include <vector>
 
 #include "common.cuh"
 
@@ -258,6 +261,20 @@ int check_tensors(const void* const* grads, const int64_t* numels, const int32_t
   return FM_OK;
 }
 
+// Refuses tensors that share memory, also with the factor: two blocks would scale it, once or twice.
+int check_apart(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, const float* factor) {
+  std::vector<std::pair<uintptr_t, uintptr_t>> r;
+  r.reserve(count + 1);
+  r.emplace_back((uintptr_t)factor, (uintptr_t)factor + 4);
+  for (int i = 0; i < count; ++i)
+    if (numels[i] > 0)
+      r.emplace_back((uintptr_t)grads[i], (uintptr_t)grads[i] + (size_t)numels[i] * dtype_bytes(dtypes[i]));
+  if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
+  for (size_t i = 1; i < r.size(); ++i)
+    if (r[i].first < r[i - 1].second) return fail(FM_ERR_INVALID, "tensors to scale overlap (the same one twice?)");
+  return FM_OK;
+}
+
 // Fills tables and hands each to `go(table)`.
 template <int N, typename Go>
 int for_tables(const void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, int chunk, Go go) {
@@ -351,6 +368,12 @@ extern "C" int fm_scale_multi(void* const* grads, const int64_t* numels, const i
   int rc = check_tensors(grads, numels, dtypes, count);
   if (rc != FM_OK) return rc;
   if (!factor || (reinterpret_cast<uintptr_t>(factor) & 3u) != 0) return fail(FM_ERR_INVALID, "null or misaligned factor");
+  try {
+    rc = check_apart(grads, numels, dtypes, count, factor);
+  } catch (...) {
+    rc = fail(FM_ERR_INVALID, "out of host memory");
+  }
+  if (rc != FM_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](const auto& tab) -> int {
     const unsigned total = tab.first[tab.count];

@@ -334,7 +334,7 @@ int fm_grad_norm(const void* const* grads, const int64_t* numels, const int32_t*
                  double max_norm, float* result, void* workspace, size_t workspace_bytes, void* stream);
 
 /* grads[i] <- round(grads[i] * *factor) for `count` tensors, in place; `factor` is a device float.  With a
- * factor of exactly 1 nothing is read or written. */
+ * factor of exactly 1 nothing is read or written.  Tensors that overlap are refused. */
 int fm_scale_multi(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count,
                    const float* factor, void* stream);
 

@@ -174,6 +174,11 @@ def test_norm_and_scale_refuse():
     assert lib.fm_scale_multi(at(ptr), at(n), at(dt), 1, None, None) == INVALID
     assert lib.fm_scale_multi(at(ptr), at(n), at(dt), -1, 0x1000, None) == INVALID
     assert lib.fm_scale_multi(None, None, None, 0, 0x1000, None) == 0
+    two = [array("Q", [0x2000, 0x1000]), array("q", [4, 2049]), array("i", [0, 0])]      # bf16: the second ends at 0x2002
+    assert lib.fm_scale_multi(*map(at, two), 2, 0x8000, None) == INVALID and b"overlap" in lib.fm_last_error()
+    two[0][1] = 0x2000
+    assert lib.fm_scale_multi(*map(at, two), 2, 0x8000, None) == INVALID
+    assert lib.fm_scale_multi(at(ptr), at(n), at(dt), 1, 0x1004, None) == INVALID        # the factor inside a tensor
 
 
 # ---------------------------------------------------------------- refusals of the Python operators

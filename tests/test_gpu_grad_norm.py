@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import flash_muon_b200 as fm
+from flash_muon_b200._lib import FlashMuonError
 from oracle import adamw_oracle as A
 
 pytestmark = pytest.mark.gpu
@@ -91,6 +92,16 @@ def test_clip_in_place(dtypes, offset):
     values[5][123] = math.nan
     assert math.isnan(float(fm.clip_grad_norm_(params, 1.0)))
     assert all(v.isnan().all() for v in values)
+
+
+def test_the_same_gradient_twice():
+    """Counted twice by the norm, which only reads; refused where it would be scaled twice."""
+    p = torch.nn.Parameter(torch.zeros(4, device=DEV))
+    p.grad = torch.full((4,), 3.0, device=DEV)
+    assert float(fm.grad_norm([p.grad, p.grad])[0]) == pytest.approx(math.sqrt(72.0), rel=1e-6)
+    with pytest.raises(FlashMuonError, match="overlap"):
+        fm.clip_grad_norm_([p, p], 1.0)
+    assert (p.grad == 3.0).all()
 
 
 def test_iterables_and_single_parameters():
