@@ -24,10 +24,10 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kEach32 = 8;         // elements per thread with 32-bit states: a tile of 1024
-constexpr int kMaxThreads = 1024;  // of a block that takes a whole small tensor
+constexpr int kMaxThreads = 512;   // of a block that takes a whole small tensor
 constexpr int kPart8 = 2048;       // 16 per thread with 8-bit states, where two threads share a block of
 constexpr int kMaxParts = 8;       // 32, and a block takes up to 8 such parts
-constexpr int kWholeParts = 4;     // parts of a whole small tensor
+constexpr int kWholeParts = 2;     // parts of a whole small tensor
 constexpr int kMaxHyper = 8;       // parameter groups of one launch
 // Tensors of one launch.  The table travels as a kernel argument, of 3, 9 or 30 KB (the limit is 32764
 // bytes): the largest costs the host 1.4 us more per launch than the smallest.
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) adamw_count_kernel(const __grid_cons
 // block of 128 threads: many small blocks keep loads, arithmetic and stores of different tiles mixed
 // where persistent blocks ran in step (524 M f32 elements 2.68 ms, so 2.10 = 6.98 TB/s; 131 M bf16 ones
 // 541 us, so 425 = 6.8 TB/s; a copy runs at 6.55).
-// kWhole: a block of up to 1024 threads takes a whole tensor.
+// kWhole: a block of up to 512 threads takes a whole tensor.
 template <typename P, typename G, bool kMaster, bool kWhole, int N>
 __global__ void __launch_bounds__(kWhole ? kMaxThreads : kThreads) adamw_kernel(const __grid_constant__ Table<N> tab) {
   __shared__ Coef s_coef;
@@ -902,7 +902,8 @@ struct Batch {
 };
 
 // Parts of a tile with 8-bit states: what a block spends on its tensor's coefficients is shared by up to
-// 8 of them, as many as leave every SM 12 blocks (5 to 7 are resident).
+// 8 of them, as many as leave every SM 12 blocks (5 to 7 are resident).  67 M bf16 elements, at an earlier
+// step of the kernel: 1 part 137 us, 2 132, 4 130, 8 129, 16 no better.
 int parts_of(long long elements) {
   const long long parts = elements / ((long long)kPart8 * 12 * sm_count() + 1);
   return parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : (int)parts;
@@ -965,8 +966,9 @@ int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cu
       works[w].largest = std::max(works[w].largest, (long long)groups[gi].numels[i]);
     }
   }
-  // One block per tensor saves the launch of the counts, 2 us, as long as a block is not much longer
-  // over a tensor than many blocks are: up to 8192 elements.
+  // One block per tensor saves the launch of the counts, 2 us of host time.  On the device that is 3.7 us
+  // instead of 4.1 for 65 tensors of 1000 f32 elements and 4.3 either way for 65 of 4096, but 6.1 instead of
+  // 5.3 for 65 of 8192 (8-bit states 4.0 / 4.8, 4.5 / 4.3, 6.3 / 4.8): up to 4096 elements.
   const auto whole = [&](const Work& w) {
     return w.largest <= (w.kind.bits == 8 ? kWholeParts * kPart8 : kMaxThreads * kEach32);
   };

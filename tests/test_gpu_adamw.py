@@ -34,7 +34,7 @@ KINDS = [(B16, B16, False), (B16, F32, False), (H16, H16, False), (H16, F32, Fal
 IDS = [f"{str(p)[6:]}-{str(g)[6:]}{'-master' if w else ''}" for p, g, w in KINDS]
 # the first list has tensors of several blocks, in the others a block takes each tensor whole
 SIZES = {"several": [1, 3, 16, 31, 32, 33, 255, 1000, 4095, 4096, 4097, 8192 + 17, 20000],
-         "whole": [1, 31, 32, 33, 1000, 2048, 2049, 4096, 5000, 8191, 8192], "one": [1000], "least": [8193]}
+         "whole": [1, 31, 32, 33, 1000, 2047, 2048, 2049, 4095, 4096], "one": [1000], "least": [4097], "short": [33, 8191, 8192]}
 HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
 
 
@@ -159,7 +159,7 @@ def test_scale_lr_tensor_and_steps_list():
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("n", [5000, 70000])
+@pytest.mark.parametrize("n", [3000, 70000])
 def test_a_factor_that_is_not_finite_takes_no_step(bad, bits, n):
     p, g = torch.randn(n, device=DEV), torch.randn(n, device=DEV)
     steps = torch.tensor([4.0], device=DEV)
@@ -175,16 +175,16 @@ def test_a_factor_that_is_not_finite_takes_no_step(bad, bits, n):
     assert all(torch.equal(a, b) for a, b in zip(before, (p, g, steps, *st)))
 
 
-@pytest.mark.parametrize("n", [4200, 12000])
+@pytest.mark.parametrize("n", [4096, 12000])
 def test_nan_and_inf_gradients_stay_where_they_are(n):
     p, g = torch.randn(n, device=DEV), torch.randn(n, device=DEV)
-    g[7], g[4100] = math.nan, math.inf
+    g[7], g[4090] = math.nan, math.inf
     m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
     fm.adamw_step([p], [g], [m], [v], torch.zeros(1, device=DEV), lr=0.1)
     ok = torch.ones(n, dtype=torch.bool, device=DEV)
-    ok[7] = ok[4100] = False
+    ok[7] = ok[4090] = False
     assert p[ok].isfinite().all() and m[ok].isfinite().all() and v[ok].isfinite().all()
-    assert p[~ok].isnan().all() and math.isinf(m[4100]) and math.isinf(v[4100]) and math.isnan(m[7])
+    assert p[~ok].isnan().all() and math.isinf(m[4090]) and math.isinf(v[4090]) and math.isnan(m[7])
 
 
 @pytest.mark.parametrize("bits", [32, 8])

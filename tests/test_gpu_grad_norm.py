@@ -33,8 +33,8 @@ def tensors(sizes, dtypes, offset=0, seed=0, size=1e-2):
 @pytest.mark.parametrize("dtypes", [[B16], [H16], [F32], [B16, F32, H16]], ids=["bf16", "f16", "f32", "mixed"])
 @pytest.mark.parametrize("offset", [0, 1, 3])
 @pytest.mark.parametrize("sizes", [[1], [7, 0, 33], [8191, 8192, 8193, 100000], [3] * 200, [500_003], [65] * 2500,
-                                   [1024] * 511 + [1000], [1024] * 511 + [1025], [1] * 512, [1023, 1024, 1025, 70_000]],
-                         ids=["one", "few", "chunks", "vectors", "long", "tables", "cluster", "past-cluster", "ones", "units"])
+                                   [1024] * 255 + [1000], [1024] * 255 + [1025], [1] * 256, [1] * 257, [1023, 1024, 1025, 70_000]],
+                         ids=["one", "few", "chunks", "vectors", "long", "tables", "cluster", "past-cluster", "ones", "past-ones", "units"])
 def test_norm_against_64_bits(dtypes, offset, sizes):
     g = tensors(sizes, dtypes, offset, len(sizes))
     keep = [x.clone() for x in g]
