@@ -52,6 +52,7 @@ struct Hyper {
   double lr, beta1, beta2, wd;
   const float* lr_dev;            // overrides lr where set
   float b1, omb1, b2, omb2, eps;  // betas, 1 - betas
+  float root_omb2;
 };
 template <int N>
 struct Table {
@@ -72,7 +73,7 @@ struct CountTable {
 
 // What depends on a tensor's step count.
 struct Coef {
-  float size, root, decay;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
+  float size, root, decay;  // lr / (1 - b1^t), sqrt(1 - b2^t), 1 - lr wd
   uint32_t key;
 };
 
@@ -138,10 +139,17 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466
 __device__ __forceinline__ bool skipped(const float* scale) { return scale != nullptr && !finite(*scale); }
 
 // Tensor of a tile.  Every thread searches for itself: the table is in constant memory, all lanes
-// read the same word, and no barrier stands before the loads of the tile.
+// read the same word, and no barrier stands before the loads of the tile.  The first tensors, where
+// the large ones mostly are, are found in the fewest steps (an embedding followed by 65 norms: 426 us,
+// so 423).
 template <typename Tab>
 __device__ __forceinline__ int find(const Tab& tab, unsigned tile) {
-  int lo = 0, hi = tab.count;
+  int lo = 0, hi = 1;
+  while (hi < tab.count && tab.first[hi] <= tile) {
+    lo = hi;
+    hi *= 2;
+  }
+  hi = min(hi, tab.count);
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (tab.first[mid] <= tile) lo = mid;
@@ -166,7 +174,7 @@ __device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, uin
       const float lr = h.lr_dev ? *h.lr_dev : (float)h.lr;
       c->size = lr / (float)(1.0 - power(h.beta1, t));
     } else if (which == 1) {
-      c->root = 1.f / sqrtf((float)(1.0 - power(h.beta2, t)));
+      c->root = sqrtf((float)(1.0 - power(h.beta2, t)));
     } else if (which == 2) {
       c->key = state8::index_key(state8::step_key(e.seed, t), index_hi);
     } else if (which == 3) {
@@ -175,6 +183,24 @@ __device__ __forceinline__ void coefficients(const Hyper& h, const Entry& e, uin
   }
   __syncthreads();
   if (whole && taken && threadIdx.x == 0) *e.step = count;  // read by all of its readers
+}
+
+// Root and reciprocal within 1 ulp.  The correctly rounded ones cost the 32-bit step 8 registers per
+// thread and 1 to 2 %.  Subnormal arguments count as zero, except for sqrt_approx.
+__device__ __forceinline__ float root_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // ---------------------------------------------------------------- step counts
@@ -234,13 +260,14 @@ __global__ void __launch_bounds__(kWhole ? kMaxThreads : kThreads) adamw_kernel(
   const float scale = tab.scale ? *tab.scale : 1.f;
   coefficients(h, e, 0, kWhole, finite(scale), &s_coef);
   if (!finite(scale)) return;
-  const Coef c = s_coef;
+  // size m / (sqrt(v) / root + eps) = size root m / (sqrt(v) + eps root)
+  const float decay = s_coef.decay, size = -s_coef.size * s_coef.root, eps = h.eps * s_coef.root;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float gr = to_f<G>(gv[j]) * scale;
     mv[j] = fmaf(h.b1, mv[j], h.omb1 * gr);
     vv[j] = fmaf(h.b2, vv[j], h.omb2 * (gr * gr));
-    wv[j] = fmaf(kMaster ? wv[j] : to_f<P>(pv[j]), c.decay, -c.size * (mv[j] / fmaf(sqrtf(vv[j]), c.root, h.eps)));
+    wv[j] = fmaf(kMaster ? wv[j] : to_f<P>(pv[j]), decay, size * (mv[j] * rcp_approx(sqrt_approx(vv[j]) + eps)));
     pv[j] = from_f<P>(wv[j]);
   }
   if (vec) {
@@ -270,9 +297,9 @@ __global__ void __launch_bounds__(kWhole ? kMaxThreads : kThreads) adamw_kernel(
 //   decode m: e4m3 pairs to f16 pairs, exact; v: the code shifted to bit 7 IS an f16 number;
 //   encode: scaled by the block's power of two (state8.cuh) the code is the bits above bit 20, the
 //   random number is added below and cut off.
-// The parts of a block's tile are copied to shared memory two ahead.  67 M bf16 elements 114 us (6.0 TB/s,
-// 91 % of a copy; 46 instructions per element, issue slots 79 % busy), f32 168 us (98 %), bf16 with masters 174 us
-// (95 %); elements at odd addresses 199 to 279 us.
+// The parts of a block's tile are copied to shared memory two ahead.  67 M bf16 elements 115 us (5.9 TB/s,
+// 90 % of a copy; 46 instructions per element, issue slots 79 % busy), f32 169 us (98 %), bf16 with masters 172 us
+// (96 %); elements at odd addresses 199 to 279 us.
 // Two cases that hardly ever occur leave this path: a block whose largest magnitude is not finite or
 // beyond what one normal fp32 factor scales, and a positive v whose code came out 0.
 typedef unsigned long long f32x2;
@@ -289,23 +316,17 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   f32x2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ f32x2 both(float x) { return pack2(x, x); }
-// within 1 ulp of the root and the reciprocal, subnormal arguments taken as zero
-__device__ __forceinline__ float root_approx(float x) {
-  float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // the largest magnitude; not a number if one of them is not
 __device__ __forceinline__ float max_abs(float a, float b, float c) {
   float r;
@@ -376,10 +397,11 @@ struct Staged {
   }
 };
 
-// Resident blocks per SM that registers are kept down for, as many as shared memory has room for.
+// Resident blocks per SM that registers are kept down for: 6, with two float32 arrays in shared memory 5.
+// A seventh of 16-bit types leaves 72 registers, which some builds spill (114 to 132 us where 6 take 115).
 template <typename W, typename G>
 constexpr int resident8() {
-  return sizeof(W) + sizeof(G) == 4 ? 7 : sizeof(W) + sizeof(G) == 6 ? 6 : 5;
+  return sizeof(W) + sizeof(G) <= 6 ? 6 : 5;
 }
 
 template <typename P, typename G, bool kMaster, int N>
@@ -457,8 +479,6 @@ __global__ void __launch_bounds__(kThreads, resident8<std::conditional_t<kMaster
       st.v.read(vq);
       st.g.read(gv);
       st.w.read(wv);
-      __syncthreads();
-      fetch(start + 2 * kPart8, stage);
     } else {  // through shared memory: neighbouring threads read neighbouring elements
       *reinterpret_cast<uint4*>(mq) = *reinterpret_cast<uint4*>(vq) = make_uint4(0, 0, 0, 0);
       if (at < coded) {
@@ -493,37 +513,47 @@ __global__ void __launch_bounds__(kThreads, resident8<std::conditional_t<kMaster
         return;
       }
     }
-    const f32x2 root = both(s_coef.root), decay = both(s_coef.decay), size = both(-s_coef.size);
-    const f32x2 b1 = both(h.b1), o1 = both(h.omb1), b2 = both(h.b2), o2 = both(h.omb2), eps = both(h.eps), sc = both(scale);
+    // the factor of the gradient goes into the constants; that of the second moment is applied before the
+    // square, which it keeps in range
+    const f32x2 decay = both(s_coef.decay), size = both(-s_coef.size * s_coef.root), eps = both(h.eps * s_coef.root);
+    const f32x2 b1 = both(h.b1), c1 = both(h.omb1 * scale), b2 = both(h.b2), c2 = both(h.root_omb2 * scale);
 
     float m[16], v[16];
-    alignas(16) float wn[16];
+    alignas(16) W wn[16];  // rounded already: half the registers for 16-bit types
     const f32x2 mf = both(factor_m(mb)), vf = both(factor_v(vb));
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
       f32x2 m2 = mul2(decode_m2(reinterpret_cast<uint32_t*>(mq)[j / 4], j & 2), mf);
       f32x2 v2 = mul2(decode_v2(reinterpret_cast<uint32_t*>(vq)[j / 4], j & 2), vf);
-      const f32x2 g2 = mul2(pack2(to_f<G>(gv[j]), to_f<G>(gv[j + 1])), sc);
-      m2 = fma2(b1, m2, mul2(o1, g2));
-      v2 = fma2(b2, v2, mul2(o2, mul2(g2, g2)));
+      const f32x2 g2 = pack2(to_f<G>(gv[j]), to_f<G>(gv[j + 1])), u2 = mul2(c2, g2);
+      m2 = fma2(b1, m2, mul2(c1, g2));
+      v2 = fma2(u2, u2, mul2(b2, v2));
       unpack2(m2, m[j], m[j + 1]);
       unpack2(v2, v[j], v[j + 1]);
       // the update takes the moments before they are rounded to 8 bits
       float d0, d1;
-      unpack2(fma2(pack2(root_approx(v[j]), root_approx(v[j + 1])), root, eps), d0, d1);
+      unpack2(add2(pack2(root_approx(v[j]), root_approx(v[j + 1])), eps), d0, d1);
       const f32x2 d2 = mul2(m2, pack2(rcp_approx(d0), rcp_approx(d1)));
       const f32x2 w2 = pack2(to_f<W>(wv[j]), to_f<W>(wv[j + 1]));
-      unpack2(fma2(w2, decay, mul2(size, d2)), wn[j], wn[j + 1]);
+      unpack2(fma2(w2, decay, mul2(size, d2)), d0, d1);
+      wn[j] = from_f<W>(d0);
+      wn[j + 1] = from_f<W>(d1);
     }
     if (vec) {
-      alignas(16) P out[16];
+      __syncthreads();  // every thread has read its elements
+      fetch(start + 2 * kPart8, stage);
+      if constexpr (kMaster) {
+        alignas(16) P out[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) out[j] = from_f<P>(wn[j]);
-      store_vec(p + at, out);
-      if (kMaster) store_vec(w + at, wn);
+        for (int j = 0; j < 16; ++j) out[j] = from_f<P>(wn[j]);
+        store_vec(p + at, out);
+        store_vec(w + at, wn);
+      } else {
+        store_vec(p + at, wn);
+      }
     } else {  // written from there below; a thread overwrites only what it alone has read
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s_w[padded(mine + j)] = wn[j];
+      for (int j = 0; j < 16; ++j) s_w[padded(mine + j)] = to_f<W>(wn[j]);
     }
     float mx = max_abs(m[0], m[1], m[2]), vx = max_abs(v[0], v[1], v[2]);
 #pragma unroll
@@ -881,6 +911,7 @@ struct Batch {
       h.eps = g.state_bits == 8 ? std::max((float)g.eps, 0x1p-64f) : (float)g.eps;
       h.b1 = (float)g.beta1; h.omb1 = (float)(1.0 - g.beta1);
       h.b2 = (float)g.beta2; h.omb2 = (float)(1.0 - g.beta2);
+      h.root_omb2 = (float)std::sqrt(1.0 - g.beta2);
       last_group = gi;
     }
     Entry& e = tab.e[tab.count];
@@ -902,7 +933,7 @@ struct Batch {
 };
 
 // Parts of a tile with 8-bit states: what a block spends on its tensor's coefficients is shared by up to
-// 8 of them, as many as leave every SM 12 blocks (5 to 7 are resident).  67 M bf16 elements, at an earlier
+// 8 of them, as many as leave every SM 12 blocks (5 or 6 are resident).  67 M bf16 elements, at an earlier
 // step of the kernel: 1 part 137 us, 2 132, 4 130, 8 129, 16 no better.
 int parts_of(long long elements) {
   const long long parts = elements / ((long long)kPart8 * 12 * sm_count() + 1);
