@@ -175,6 +175,9 @@ grad_norm_small_kernel(const __grid_constant__ Table<N> tab, double max_norm, fl
   namespace cg = cooperative_groups;
   __shared__ double red[kClusterThreads / 32], all[kCluster];
   const cg::cluster_group cluster = cg::this_cluster();
+  // A block's shared memory may be written from outside only once the block runs: all say so here, and
+  // the wait stands in front of the write, behind the loads.
+  cluster.barrier_arrive();
   const unsigned total = tab.first[tab.count];
   const int warp = threadIdx.x >> 5;
   double s = 0.0;
@@ -191,6 +194,7 @@ grad_norm_small_kernel(const __grid_constant__ Table<N> tab, double max_norm, fl
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) red[warp] = s;
   __syncthreads();
+  cluster.barrier_wait();
   if (threadIdx.x == 0) {
     for (int i = 1; i < kClusterThreads / 32; ++i) s += red[i];
     cluster.map_shared_rank(all, 0)[blockIdx.x] = s;
