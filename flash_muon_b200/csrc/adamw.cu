@@ -343,9 +343,8 @@ __device__ __forceinline__ uint32_t at_most_inf(uint32_t h2) {
   asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h2), "r"(0x7c007c00u));
   return r;
 }
-// Codes of a word (the upper two where `upper`) without their block's factor, and the factors:
-// 2^(b - 134) and 2^(b - 141) times the codes read as e4m3 and f16.  Fresh states have scale byte 0 and
-// only zero codes.
+// Codes of a word (the upper two where `upper`) read as e4m3 and f16, without their block's factor
+// (state8.cuh).  Fresh states have scale byte 0 and only zero codes.
 __device__ __forceinline__ f32x2 decode_m2(uint32_t w, bool upper) {
   uint32_t h2;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((unsigned short)(upper ? w >> 16 : w)));
@@ -355,8 +354,6 @@ __device__ __forceinline__ f32x2 decode_v2(uint32_t w, bool upper) {
   // code 255, infinity, comes out of the shift as "not a number"
   return halves_to_floats(at_most_inf(__byte_perm(w, 0, upper ? 0x4342 : 0x4140) << 7));
 }
-__device__ __forceinline__ float factor_m(int b) { return state8::pow2(max(b, state8::kMinExpM) - 7); }
-__device__ __forceinline__ float factor_v(int b) { return state8::pow2(max(b, state8::kMinExpV) - 14); }
 // A word of padding per 16: a thread's 16 elements and a warp's neighbouring ones are both free of
 // bank conflicts.
 __device__ __forceinline__ int padded(int i) { return i + (i >> 4); }
@@ -520,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, resident8<std::conditional_t<kMaster
 
     float m[16], v[16];
     alignas(16) W wn[16];  // rounded already: half the registers for 16-bit types
-    const f32x2 mf = both(factor_m(mb)), vf = both(factor_v(vb));
+    const f32x2 mf = both(state8::factor_m(mb)), vf = both(state8::factor_v(vb));
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
       f32x2 m2 = mul2(decode_m2(reinterpret_cast<uint32_t*>(mq)[j / 4], j & 2), mf);
@@ -661,7 +658,7 @@ adamw8_values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int
   if (vec && at + 32 <= n) {
     alignas(32) uint8_t c[32];
     load_vec(codes + at, c);
-    const f32x2 factor = both(kMoment == 1 ? factor_m(b) : factor_v(b));
+    const f32x2 factor = both(kMoment == 1 ? state8::factor_m(b) : state8::factor_v(b));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // 16 at a time: fewer registers
       alignas(32) T x[16];
@@ -677,8 +674,11 @@ adamw8_values_kernel(const uint8_t* codes, const uint8_t* exps, long long n, int
     }
     return;
   }
-  for (int j = 0; j < 32 && at + j < n; ++j)
-    out[at + j] = from_f<T>(kMoment == 1 ? state8::decode_m(codes[at + j], b) : state8::decode_v(codes[at + j], b));
+  for (int j = 0; j < 32 && at + j < n; ++j) {
+    const uint8_t c = codes[at + j];
+    out[at + j] = from_f<T>(kMoment == 1 ? state8::decode_m(c, b)
+                                         : state8::decode_v(c >= state8::kInfiniteV ? (uint8_t)255 : c, b));
+  }
 }
 
 // One warp per block of 32, rounding to nearest.

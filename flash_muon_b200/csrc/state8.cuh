@@ -33,6 +33,9 @@ namespace state8 {
 constexpr int kBlock = 32;
 // Range of the exponent byte: from 17 and 32 on the smallest code of a block is a normal fp32 number.
 constexpr int kMinExpM = 17, kMinExpV = 32, kMaxExp = 253;
+// Second-moment codes from here on are only written where they stand for infinity (a largest element beyond 2^126
+// leaves the binade of its exponent byte); the kernels, which read codes as f16 bits, take them all for it.
+constexpr int kInfiniteV = 248;
 constexpr uint32_t kNearest = 1u << 19;                   // the "random" number of rounding to nearest
 
 FM_HD uint32_t bits_of(float x) {
@@ -98,15 +101,19 @@ FM_HD uint8_t encode_v(float x, int b, uint32_t r) {
   if (c == 0) return mag != 0 ? 1 : 0;
   return (uint8_t)(c > 254u ? 254u : c);
 }
+// Factors of a block's codes read as numbers with the exponent offsets 7 (e4m3) and 15 (e5m3): 2^(b - 134)
+// and 2^(b - 141).  An exponent byte below the smallest counts as the smallest.
+FM_HD float factor_m(int b) { return pow2((b > kMinExpM ? b : kMinExpM) - 7); }
+FM_HD float factor_v(int b) { return pow2((b > kMinExpV ? b : kMinExpV) - 14); }
 FM_HD float decode_m(uint8_t c, int b) {
   const uint32_t mag = c & 127u;
   if (mag == 127u) return float_of(0x7fc00000u);
-  const float x = float_of(mag << 20) * pow2(240) * pow2(b);
+  const float x = float_of(mag << 20) * pow2(247) * factor_m(b);
   return (c & 128u) ? -x : x;
 }
 FM_HD float decode_v(uint8_t c, int b) {
   if (c == 255u) return float_of(0x7f800000u);
-  return float_of((uint32_t)c << 20) * pow2(225) * pow2(b);
+  return float_of((uint32_t)c << 20) * pow2(239) * factor_v(b);
 }
 
 }  // namespace state8

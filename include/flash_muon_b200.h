@@ -269,12 +269,13 @@ int fm_muon_step(const fm_muon_group* groups, int ngroups, void* const* workspac
  * state_bits 8: they are 16-byte aligned codes, one byte per element, padded to a multiple of 32
  * bytes; exp_avg_scale[i] and exp_avg_sq_scale[i] hold one byte per 32 elements.  All zero bytes are
  * zero moments.  First moment: sign | e4m3 times 2^(scale - 134); second: unsigned e5m3 times
- * 2^(scale - 127) in units where code 248 is 1.  Codes are rounded up or down at random with the
- * chance of the distance; the random numbers are a function of seeds[i], the step count and the
- * element's index, so equal calls give equal bits.  A value that is not finite becomes "not a
- * number" (first moment, code 127) or infinity (second, code 255) and leaves its neighbours alone.
- * Scales are at least 17 (first moment) and 32 (second); a positive second moment is never stored
- * as zero; eps below 2^-64 counts as 2^-64.
+ * 2^(scale - 127) in units where code 232 is 1; codes from 248 on count as infinity.  Codes are
+ * rounded up or down at random with the chance of the distance; the random numbers are a function of
+ * seeds[i], the step count and the element's index, so equal calls give equal bits.  A value that is
+ * not finite becomes "not a number" (first moment, code 127) or infinity (second, code 255) and leaves
+ * its neighbours alone.  Scales are written from 17 (first moment) and 32 (second) to 253, and a byte
+ * below that range counts as its lower end; a positive second moment is never stored as zero; eps
+ * below 2^-64 counts as 2^-64.
  */
 typedef struct {
   void* const* params;
