@@ -1080,6 +1080,7 @@ extern "C" int fm_adamw8_values(const void* codes, const void* scales, int64_t n
   int rc = check_moment(codes, scales, out, n, moment);
   if (rc != FM_OK) return rc;
   if (out_dtype < FM_BF16 || out_dtype > FM_F32) return fail(FM_ERR_UNSUPPORTED, "unknown dtype %d", out_dtype);
+  if (!aligned(out, dtype_bytes(out_dtype))) return fail(FM_ERR_INVALID, "misaligned values");
   if (n == 0) return FM_OK;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
@@ -1105,6 +1106,7 @@ extern "C" int fm_adamw8_encode(const void* values, int v_dtype, int64_t n, int 
   int rc = check_moment(values, codes, scales, n, moment);
   if (rc != FM_OK) return rc;
   if (v_dtype < FM_BF16 || v_dtype > FM_F32) return fail(FM_ERR_UNSUPPORTED, "unknown dtype %d", v_dtype);
+  if (!aligned(values, dtype_bytes(v_dtype))) return fail(FM_ERR_INVALID, "misaligned values");
   if (n == 0) return FM_OK;
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* s = static_cast<uint8_t*>(scales);
