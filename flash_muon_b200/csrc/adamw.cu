@@ -907,11 +907,14 @@ struct Batch {
       Hyper& h = tab.h[hypers++];
       h.lr = g.lr; h.beta1 = g.beta1; h.beta2 = g.beta2; h.lr_dev = g.lr_device;
       h.wd = g.weight_decay;
-      // the smallest stored second moment is 2^-126; a step may leave less, whose approximate root is 0
-      h.eps = g.state_bits == 8 ? std::max((float)g.eps, 0x1p-64f) : (float)g.eps;
       h.b1 = (float)g.beta1; h.omb1 = (float)(1.0 - g.beta1);
       h.b2 = (float)g.beta2; h.omb2 = (float)(1.0 - g.beta2);
       h.root_omb2 = (float)std::sqrt(1.0 - g.beta2);
+      // 8 bits: the smallest stored second moment is 2^-126; a step may leave less, whose approximate root is 0.
+      // 32 bits: eps sqrt(1 - b2^t) >= eps sqrt(1 - b2) stays a normal number, or the approximate reciprocal
+      // were infinite where there never was a gradient.
+      const float least = g.state_bits == 8 ? 0x1p-64f : g.eps > 0.0 ? 0x1p-125f / h.root_omb2 : 0.f;
+      h.eps = std::max((float)g.eps, least);
       last_group = gi;
     }
     Entry& e = tab.e[tab.count];

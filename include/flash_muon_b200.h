@@ -305,7 +305,7 @@ typedef struct {
  *   g' = s g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
  *   w = w (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * in fp32, each stored value rounded once; 8-bit moments enter w before they are rounded.  Root and
- * reciprocal are good to 1 ulp; a subnormal eps counts as zero.
+ * reciprocal are good to 1 ulp; a positive eps counts as 2^-125 / sqrt(1 - b2) at least.
  * grad_scale (may be null: 1) is a device float, e.g. the factor fm_grad_norm leaves; if it is not
  * finite the step is not taken: nothing is written, the counts included.
  * Tensors of one kind (types, masters, state bits) share launches, up to 360 tensors and 8 groups

@@ -20,3 +20,20 @@ def test_values_do_not_depend_on_where_a_block_lies(b, moment):
         part = fm.adamw8_values(codes, scales, moment=moment, numel=31, dtype=F32)
         assert torch.equal(whole[:31].isnan(), part.isnan())
         assert torch.equal(whole[:31].nan_to_num(nan=7.0), part.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("n", [100, 5000])
+@pytest.mark.parametrize("eps", [1e-37, 2e-38, 1e-40, 1e-60])
+def test_any_positive_eps_keeps_the_division_by_zero_away(n, eps):
+    """eps sqrt(1 - b2^t) is 3e-39 and less here, no normal number.  Elements without gradient have a zero
+    update; beside the root of any other second moment, 4e-23 at least, such an eps vanishes."""
+    g = torch.zeros(n, device=DEV)
+    g[::3] = torch.linspace(-1, 1, len(g[::3]), device=DEV) + 0.01
+    out = []
+    for e in (eps, 0.0):
+        p, m, v, steps = torch.ones(n, device=DEV), torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), torch.zeros(1, device=DEV)
+        for _ in range(2):
+            fm.adamw_step([p], [g], [m], [v], steps, lr=0.1, weight_decay=0.0, eps=e)
+        out.append(p)
+    assert (out[0][g == 0] == 1).all()
+    assert torch.equal(out[0][g != 0], out[1][g != 0]) and out[0].isfinite().all()
