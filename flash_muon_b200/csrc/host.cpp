@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cctype>
@@ -273,8 +274,8 @@ PyObject* guarded(Body body) {
   try {
     return body();
   } catch (const Refused&) {
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {
+    torch::translate_exception_to_python(std::current_exception());  // torch.OutOfMemoryError stays what it is
   } catch (...) {
     PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
   }

@@ -37,3 +37,17 @@ def test_any_positive_eps_keeps_the_division_by_zero_away(n, eps):
         out.append(p)
     assert (out[0][g == 0] == 1).all()
     assert torch.equal(out[0][g != 0], out[1][g != 0]) and out[0].isfinite().all()
+
+
+def test_out_of_memory_is_torch_s_own_error():
+    """The allocator's limit for this process is lowered; the device has memory left."""
+    codes, scales = torch.zeros(1 << 28, dtype=torch.uint8, device=DEV), torch.zeros(1 << 23, dtype=torch.uint8, device=DEV)
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(DEV).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            fm.adamw8_values(codes, scales, moment=1, dtype=F32)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert fm.adamw8_values(codes, scales, moment=1, numel=100, dtype=F32).numel() == 100
