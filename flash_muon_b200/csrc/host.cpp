@@ -14,6 +14,7 @@
 
 #include <cctype>
 #include <cmath>
+#include <deque>
 #include <optional>
 #include <string>
 #include <vector>
@@ -90,18 +91,25 @@ double number(PyObject* o) {
   return x;
 }
 
+// Tells autograd that a tensor was written: a backward pass that saved it is refused.
+void mark_written(c10::TensorImpl* t) {
+  if (!t->is_inference()) t->bump_version();
+}
+
 // One parameter group of a call, in arrays that live until the call returns.
 struct Group {
   std::vector<int64_t> numels;
   std::vector<void*> params, grads, masters, m, v, ms, vs, steps;
   std::vector<uint32_t> seeds;
+  std::vector<c10::TensorImpl*> written;
   fm_adamw_group g;
 };
 
 // What a parameter is stepped with; master, scales may be null.
 struct Row {
   const at::Tensor *p, *grad, *master, *m, *v, *ms, *vs;
-  void* step;
+  void* step;               // the count, and the tensor that holds it
+  const at::Tensor* count;
   uint32_t seed;
 };
 
@@ -155,6 +163,10 @@ class Builder {
       x.vs.push_back(r.vs->data_ptr());
       x.seeds.push_back(r.seed);
     }
+    for (const at::Tensor* t : {r.p, r.m, r.v, r.master, r.ms, r.vs})
+      if (t) x.written.push_back(t->unsafeGetTensorImpl());
+    c10::TensorImpl* const count = r.count->unsafeGetTensorImpl();
+    if (count != last_count_) x.written.push_back(last_count_ = count);  // one tensor may hold them all
   }
 
  private:
@@ -182,6 +194,7 @@ class Builder {
     x.g.state_bits = eight ? 8 : 32;
     for (std::vector<void*>* v : {&x.params, &x.grads, &x.m, &x.v, &x.steps}) v->reserve(expected);
     x.numels.reserve(expected);
+    x.written.reserve(expected * (eight ? 6 : 4) + (master ? expected : 0));
     if (master) x.masters.reserve(expected);
     if (eight) {
       x.ms.reserve(expected);
@@ -195,6 +208,7 @@ class Builder {
   const size_t first_;
   const int device_;
   const fm_adamw_group settings_;
+  c10::TensorImpl* last_count_ = nullptr;
 };
 
 void learning_rate(PyObject* lr, int device, fm_adamw_group& g) {
@@ -209,18 +223,19 @@ uint32_t seed_of(PyObject* o) {
 }
 
 // (params, grads, masters, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, steps, seeds, lr, beta1,
-// beta2, eps, weight_decay); masters, scales and seeds may be None.
-void parse_group(PyObject* tuple, int& device, std::vector<Group>& out) {
+// beta2, eps, weight_decay); masters, scales and seeds may be None.  `keep` holds the tensors until the call
+// returns.
+void parse_group(PyObject* tuple, int& device, std::vector<Group>& out, std::deque<Items>& keep) {
   const Items f(tuple, "group");
   REQUIRE(f.size() == 14, "a group has 14 entries");
-  const Items params(f[0], "params"), grads(f[1], "grads");
+  const Items &params = keep.emplace_back(f[0], "params"), &grads = keep.emplace_back(f[1], "grads");
   const Py_ssize_t n = params.size();
   if (n == 0) return;
   const bool eight = f[5] != Py_None, master = f[2] != Py_None;
-  const Items m(f[3], "exp_avgs"), v(f[4], "exp_avg_sqs");
-  std::optional<Items> w, ms, vs, seeds, steps;
-  auto list = [&](std::optional<Items>& items, int k, const char* name) {
-    items.emplace(f[k], name);
+  const Items &m = keep.emplace_back(f[3], "exp_avgs"), &v = keep.emplace_back(f[4], "exp_avg_sqs");
+  const Items *w = nullptr, *ms = nullptr, *vs = nullptr, *seeds = nullptr, *steps = nullptr;
+  auto list = [&](const Items*& items, int k, const char* name) {
+    items = &keep.emplace_back(f[k], name);
     return items->size() == n;
   };
   bool same = grads.size() == n && m.size() == n && v.size() == n;
@@ -248,13 +263,14 @@ void parse_group(PyObject* tuple, int& device, std::vector<Group>& out) {
   Builder rows(out, device, g);
   for (Py_ssize_t i = 0; i < n; ++i) {
     Row r = {&tensor(params[i], "params"), &tensor(grads[i], "grads"), master ? &tensor((*w)[i], "masters") : nullptr,
-             &tensor(m[i], "exp_avgs"), &tensor(v[i], "exp_avg_sqs"), nullptr, nullptr, nullptr, 0};
+             &tensor(m[i], "exp_avgs"), &tensor(v[i], "exp_avg_sqs"), nullptr, nullptr, nullptr, nullptr, 0};
     if (eight) {
       r.ms = &tensor((*ms)[i], "exp_avg_scales");
       r.vs = &tensor((*vs)[i], "exp_avg_sq_scales");
       r.seed = seed_of((*seeds)[i]);
     }
-    r.step = steps ? step_count(tensor((*steps)[i], "steps"), device) : counts + i;
+    r.count = steps ? &tensor((*steps)[i], "steps") : &THPVariable_Unpack(f[7]);
+    r.step = steps ? step_count(*r.count, device) : counts + i;
     rows.add(r, n);
   }
 }
@@ -309,7 +325,11 @@ int launch(decltype(&fm_adamw_step) fn, std::vector<Group>& groups, int device, 
     table.push_back(x.g);
   }
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
-  return fn(table.data(), (int)table.size(), scale, c10::cuda::getCurrentCUDAStream().stream());
+  const int rc = fn(table.data(), (int)table.size(), scale, c10::cuda::getCurrentCUDAStream().stream());
+  if (rc == FM_OK)
+    for (const Group& x : groups)
+      for (c10::TensorImpl* t : x.written) mark_written(t);
+  return rc;
 }
 
 // adamw_step(fm_adamw_step, groups, grad_scale or None) -> status
@@ -318,10 +338,11 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     need(n, 3);
     const auto fn = entry<decltype(&fm_adamw_step)>(a[0]);
     const Items tuples(a[1], "groups");
+    std::deque<Items> keep;
     std::vector<Group> groups;
     groups.reserve(tuples.size() + 4);
     int device = -1;
-    for (Py_ssize_t i = 0; i < tuples.size(); ++i) parse_group(tuples[i], device, groups);
+    for (Py_ssize_t i = 0; i < tuples.size(); ++i) parse_group(tuples[i], device, groups, keep);
     return PyLong_FromLong(launch(fn, groups, device, a[2]));
   });
 }
@@ -416,9 +437,10 @@ PyObject* optimizer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
           return x ? &tensor(x, name) : nullptr;
         };
         Row r = {&p, &grad, get(k_master, "masters", false), get(k_m, "exp_avgs", true), get(k_v, "exp_avg_sqs", true),
-                 get(k_ms, "exp_avg_scales", false), nullptr, nullptr, (uint32_t)(seed + (uint32_t)index)};
+                 get(k_ms, "exp_avg_scales", false), nullptr, nullptr, get(k_step, "steps", true),
+                 (uint32_t)(seed + (uint32_t)index)};
         if (r.ms) r.vs = get(k_vs, "exp_avg_sq_scales", true);
-        r.step = step_count(*get(k_step, "steps", true), device);
+        r.step = step_count(*r.count, device);
         rows->add(r, params.size());
       }
     }
@@ -488,8 +510,11 @@ PyObject* scale(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Gradients g(grads);
     const float* factor = static_cast<const float*>(scalar(a[2], "factor", g.device));
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)g.device);
-    return PyLong_FromLong(fn(g.at.data(), g.numels.data(), g.dtypes.data(), (int)g.at.size(), factor,
-                              c10::cuda::getCurrentCUDAStream().stream()));
+    const int rc = fn(g.at.data(), g.numels.data(), g.dtypes.data(), (int)g.at.size(), factor,
+                      c10::cuda::getCurrentCUDAStream().stream());
+    if (rc == FM_OK)
+      for (Py_ssize_t i = 0; i < grads.size(); ++i) mark_written(tensor(grads[i], "grads").unsafeGetTensorImpl());
+    return PyLong_FromLong(rc);
   });
 }
 

@@ -51,3 +51,61 @@ def test_out_of_memory_is_torch_s_own_error():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert fm.adamw8_values(codes, scales, moment=1, numel=100, dtype=F32).numel() == 100
+
+
+def test_a_backward_pass_over_what_was_written_is_refused():
+    """The step and the scaling raise the version counters of what they write, and of nothing else."""
+    w = torch.nn.Parameter(torch.randn(100, device=DEV))
+    w.grad = torch.randn_like(w)
+    saved = (w * w).sum()
+    fm.AdamW([w]).step()
+    with pytest.raises(RuntimeError, match="inplace"):
+        saved.backward()
+    factor = torch.ones(100, device=DEV, requires_grad=True)
+    saved = (factor * w.grad).sum()
+    fm.clip_grad_norm_([w], 1e-3)
+    with pytest.raises(RuntimeError, match="inplace"):
+        saved.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("listed", [False, True], ids=["1-D steps", "list of steps"])
+def test_version_counters(bits, listed):
+    sizes = (100, 5000, 0)
+    new = lambda dt, f=lambda n: n: [torch.zeros(f(n), dtype=dt, device=DEV) for n in sizes]  # noqa: E731
+    p, g, w = new(torch.bfloat16), new(torch.bfloat16), new(F32)
+    steps = [torch.zeros((), device=DEV) for _ in sizes] if listed else torch.zeros(len(sizes), device=DEV)
+    blocks, byte = lambda n: -(-n // 32), torch.uint8  # noqa: E731
+    padded = lambda n: 32 * blocks(n)  # noqa: E731
+    st = [new(F32), new(F32)] if bits == 32 else [new(byte, padded), new(byte, blocks), new(byte, padded), new(byte, blocks)]
+    step = fm.adamw_step if bits == 32 else fm.adamw8_step
+    written = [*p, *w, *(steps if listed else [steps]), *(x for xs in st for x in xs)]
+    before = [x._version for x in written]
+    step(p, g, *st, steps, masters=w, lr=0.1)
+    assert [x._version for x in written] == [v + 1 for v in before]
+    assert all(x._version == 0 for x in g)
+    with pytest.raises(AssertionError):
+        step(p, g[::-1], *st, steps, masters=w, lr=0.1)
+    with pytest.raises(fm._lib.FlashMuonError):
+        step(p, p, *st, steps, masters=w, lr=0.1)
+    assert [x._version for x in written] == [v + 1 for v in before]
+
+
+def test_inference_tensors_are_stepped_too():
+    """They have no version counters."""
+    with torch.inference_mode():
+        p, g, m, v, steps = (torch.ones(n, device=DEV) for n in (100, 100, 100, 100, 1))
+    fm.adamw_step([p], [g], [m], [v], steps, lr=0.1)
+    with torch.inference_mode():
+        fm.adamw_step([p], [g], [m], [v], steps, lr=0.1)
+        q = torch.nn.Parameter(p)
+        q.grad = g
+        fm.clip_grad_norm_([q], 1.0)
+    assert float(steps) == 3.0 and float(g[0]) == pytest.approx(0.1, rel=1e-6)
+
+
+def test_tensors_given_by_iterators():
+    p, g, m, v = ([torch.ones(n, device=DEV) for n in (100, 5000)] for _ in range(4))
+    steps = torch.zeros(2, device=DEV)
+    fm.adamw_step(iter(p), iter(g), iter(m), (x for x in v), iter(steps.unbind()), lr=0.1)
+    assert steps.tolist() == [1.0, 1.0] and all((x < 1).all() for x in p)
