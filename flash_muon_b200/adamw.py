@@ -52,6 +52,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                masters: Sequence[Tensor] | None = None, grad_scale: Tensor | None = None) -> None:
     """One AdamW step of every tensor, in place, moments in float32.
 
+    Gradients, moments and masters have their parameter's shape, or are flat.
     ``steps`` holds a float32 count per tensor (a 1-D tensor or a list of scalars); the call adds one
     to each.  ``masters`` are float32 copies of 16-bit parameters that carry the bits those lose.
     ``grad_scale``, a float32 scalar on the device, multiplies the gradients; if it is not finite

@@ -120,6 +120,13 @@ void* step_count(const at::Tensor& t, int device) {
   return t.data_ptr();
 }
 
+// A tensor that goes element by element with a parameter has its shape; the order of the elements is as
+// clear where one of the two is flat.
+void check_sizes(const at::Tensor& t, const char* name, const at::Tensor& p) {
+  REQUIRE(t.numel() == p.numel() && (t.sizes() == p.sizes() || t.dim() == 1 || p.dim() == 1),
+          "`%s` must have the parameters' sizes, or be flat", name);
+}
+
 // Takes the rows of one parameter group, checks them and sorts them by kind (types, masters, state bits).
 class Builder {
  public:
@@ -135,18 +142,18 @@ class Builder {
     check_place(*r.p, "params", device_);
     check_place(*r.grad, "grads", device_);
     const int64_t n = r.p->numel(), blocks = (n + 31) / 32;
-    REQUIRE(r.grad->numel() == n, "`grads` must have the parameters' sizes");
+    check_sizes(*r.grad, "grads", *r.p);
     const int pd = dtype_code(r.p->scalar_type()), gd = dtype_code(r.grad->scalar_type());
     const bool eight = r.ms != nullptr;
-    moment(*r.m, "exp_avgs", eight, n, blocks);
-    moment(*r.v, "exp_avg_sqs", eight, n, blocks);
+    moment(*r.m, "exp_avgs", eight, *r.p, blocks);
+    moment(*r.v, "exp_avg_sqs", eight, *r.p, blocks);
     if (eight) {
       scales(*r.ms, "exp_avg_scales", blocks);
       scales(*r.vs, "exp_avg_sq_scales", blocks);
     }
     if (r.master) {
       check_place(*r.master, "masters", device_);
-      REQUIRE(r.master->numel() == n, "`masters` must have the parameters' sizes");
+      check_sizes(*r.master, "masters", *r.p);
       REQUIRE(r.master->scalar_type() == at::kFloat, "`masters` must be torch.float32");
       REQUIRE(pd != FM_F32, "float32 parameters have no master copies");
     }
@@ -170,11 +177,11 @@ class Builder {
   }
 
  private:
-  void moment(const at::Tensor& t, const char* name, bool eight, int64_t n, int64_t blocks) {
+  void moment(const at::Tensor& t, const char* name, bool eight, const at::Tensor& p, int64_t blocks) {
     check_place(t, name, device_);
     REQUIRE(t.scalar_type() == (eight ? at::kByte : at::kFloat), "`%s` must be torch.%s", name, eight ? "uint8" : "float32");
     if (eight) REQUIRE(t.numel() == blocks * 32, "`%s` must have one byte per element, padded to 32", name);
-    else REQUIRE(t.numel() == n, "`%s` must have the parameters' sizes", name);
+    else check_sizes(t, name, p);
   }
   void scales(const at::Tensor& t, const char* name, int64_t blocks) {
     check_place(t, name, device_);

@@ -109,3 +109,23 @@ def test_tensors_given_by_iterators():
     steps = torch.zeros(2, device=DEV)
     fm.adamw_step(iter(p), iter(g), iter(m), (x for x in v), iter(steps.unbind()), lr=0.1)
     assert steps.tolist() == [1.0, 1.0] and all((x < 1).all() for x in p)
+
+
+def test_shapes_that_do_not_fit_are_refused():
+    """As many elements in another shape are another order of the elements; flat ones have but one."""
+    z = lambda *shape: torch.zeros(shape, device=DEV)  # noqa: E731
+    half = torch.zeros(4, 16, device=DEV, dtype=torch.bfloat16)
+    ok = dict(params=[half], grads=[z(4, 16)], exp_avgs=[z(4, 16)], exp_avg_sqs=[z(4, 16)], masters=[z(4, 16)], steps=z(1), lr=0.1)
+    for name in ("grads", "exp_avgs", "exp_avg_sqs", "masters"):
+        for shape in ((16, 4), (8, 8), (4, 16, 1), (2, 2, 16)):
+            with pytest.raises(AssertionError, match=f"`{name}` must have the parameters' sizes"):
+                fm.adamw_step(**{**ok, name: [z(*shape)]})
+        fm.adamw_step(**{**ok, name: [z(64)]})
+    fm.adamw_step(**{**ok, "params": [half.view(-1)]})
+    fm.adamw_step(**ok)
+    assert float(ok["steps"]) == 6.0
+    codes = [torch.zeros(n, dtype=torch.uint8, device=DEV) for n in (64, 2, 64, 2)]
+    with pytest.raises(AssertionError, match="`grads` must have"):
+        fm.adamw8_step([half], [z(16, 4)], *[[c] for c in codes], z(1), lr=0.1)
+    scalar = z()
+    fm.adamw_step([scalar], [z(1)], [z()], [z(1)], z(1), lr=0.1)
