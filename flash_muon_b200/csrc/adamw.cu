@@ -706,42 +706,89 @@ struct Range {
   bool written;
 };
 
+// The lists of a group that name memory: where each tensor lies and how many bytes it has there.
+template <typename Visit>
+void for_lists(const fm_adamw_group& g, Visit visit) {
+  const bool eight = g.state_bits == 8;
+  const auto list = [&](const auto* at, bool written, auto bytes) {
+    visit(g.count, written, [=, &g](int i) -> Range {
+      const size_t n = (size_t)g.numels[i];
+      const uintptr_t begin = (uintptr_t)at[i];
+      return {begin, begin + bytes(n), written};
+    });
+  };
+  const auto each = [](size_t unit) { return [unit](size_t n) { return n * unit; }; };
+  const auto codes = [](size_t n) { return (n + 31) / 32 * 32; };
+  const auto scales = [](size_t n) { return (n + 31) / 32; };
+  list(g.params, true, each(dtype_bytes(g.p_dtype)));
+  list(g.grads, false, each(dtype_bytes(g.g_dtype)));
+  for (void* const* moments : {g.exp_avg, g.exp_avg_sq})
+    if (eight) list(moments, true, codes);
+    else list(moments, true, each(4));
+  if (g.masters) list(g.masters, true, each(4));
+  if (eight) {
+    list(g.exp_avg_scale, true, scales);
+    list(g.exp_avg_sq_scale, true, scales);
+  }
+  list(g.steps, true, [](size_t) { return (size_t)4; });
+  if (g.lr_device) visit(1, false, [&](int) -> Range { return {(uintptr_t)g.lr_device, (uintptr_t)g.lr_device + 4, false}; });
+}
+
 // Refuses a call whose written memory overlaps anything else of the call: two threads would race.
-// `runs`: where each list of tensors begins in r.  Lists are mostly in the order of their addresses
-// already.  Where they also lie apart from one another neighbours are all there is to compare, else
-// the sorted lists are merged.
-int check_ranges(std::vector<Range>& r, const std::vector<size_t>& runs) {
-  const auto overlap = [] { return fail(FM_ERR_INVALID, "tensors of the step overlap (the same parameter twice?)"); };
+// Where the lists are in the order of their addresses and lie apart from one another, neighbours are all there is to
+// compare; else all of it is sorted.
+int check_ranges(const fm_adamw_group* groups, int ngroups, const float* scale) {
   const auto less = [](const Range& a, const Range& b) { return a.begin < b.begin; };
   std::vector<Range> hulls;
-  hulls.reserve(runs.size());
-  for (size_t i = 0; i < runs.size(); ++i) {
-    const size_t from = runs[i], to = i + 1 < runs.size() ? runs[i + 1] : r.size();
-    if (from == to) continue;
-    if (!std::is_sorted(r.begin() + from, r.begin() + to, less)) std::sort(r.begin() + from, r.begin() + to, less);
-    Range hull = r[from];
-    for (size_t k = from + 1; k < to; ++k) {
-      if (hull.written && r[k].begin < hull.end) return overlap();
-      hull.end = std::max(hull.end, r[k].end);
-    }
-    hulls.push_back(hull);
-  }
-  std::sort(hulls.begin(), hulls.end(), less);
+  hulls.reserve(ngroups * 9 + 1);
   bool apart = true;
-  for (size_t i = 1; i < hulls.size(); ++i) apart = apart && hulls[i - 1].end <= hulls[i].begin;
-  if (apart) return FM_OK;
-  for (size_t i = 1; i < runs.size(); ++i)
-    std::inplace_merge(r.begin(), r.begin() + runs[i], i + 1 < runs.size() ? r.begin() + runs[i + 1] : r.end(), less);
+  size_t total = 1;
+  for (int gi = 0; gi < ngroups; ++gi) {
+    if (groups[gi].count == 0) continue;
+    for_lists(groups[gi], [&](int count, bool written, auto at) {
+      total += count;
+      Range hull = {0, 0, written};
+      for (int i = 0; i < count && apart; ++i) {
+        const Range x = at(i);
+        if (x.begin == x.end) continue;
+        if (hull.end == 0) hull.begin = x.begin;
+        apart = x.begin >= hull.end;
+        hull.end = x.end;
+      }
+      if (hull.end != 0) hulls.push_back(hull);
+    });
+  }
+  if (scale) hulls.push_back({(uintptr_t)scale, (uintptr_t)scale + 4, false});
+  if (apart) {
+    std::sort(hulls.begin(), hulls.end(), less);
+    for (size_t i = 1; i < hulls.size(); ++i) apart = apart && hulls[i - 1].end <= hulls[i].begin;
+    if (apart) return FM_OK;
+  }
+  std::vector<Range> r;
+  r.reserve(total);
+  if (scale) r.push_back({(uintptr_t)scale, (uintptr_t)scale + 4, false});
+  for (int gi = 0; gi < ngroups; ++gi) {
+    if (groups[gi].count == 0) continue;
+    for_lists(groups[gi], [&](int count, bool, auto at) {
+      const size_t from = r.size();
+      for (int i = 0; i < count; ++i) {
+        const Range x = at(i);
+        if (x.begin != x.end) r.push_back(x);
+      }
+      if (!std::is_sorted(r.begin() + from, r.end(), less)) std::sort(r.begin() + from, r.end(), less);
+      std::inplace_merge(r.begin(), r.begin() + from, r.end(), less);
+    });
+  }
   uintptr_t any = 0, written = 0;
   for (const Range& x : r) {
-    if (x.begin < (x.written ? any : written)) return overlap();
+    if (x.begin < (x.written ? any : written)) return fail(FM_ERR_INVALID, "tensors of the step overlap (the same parameter twice?)");
     any = std::max(any, x.end);
     if (x.written) written = std::max(written, x.end);
   }
   return FM_OK;
 }
 
-int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges, std::vector<size_t>& runs) {
+int check_group(const fm_adamw_group& g, int gi) {
   if (g.count < 0) return fail(FM_ERR_INVALID, "group %d: negative count", gi);
   if (g.count == 0) return FM_OK;
   if (!g.params || !g.grads || !g.exp_avg || !g.exp_avg_sq || !g.steps || !g.numels)
@@ -761,7 +808,7 @@ int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges, std
     return fail(FM_ERR_INVALID, "group %d: betas must lie in [0, 1)", gi);
   if (!(g.eps >= 0.0) || !std::isfinite(g.eps) || !std::isfinite(g.weight_decay) || !std::isfinite(g.lr))
     return fail(FM_ERR_INVALID, "group %d: lr, eps and weight_decay must be finite, eps not negative", gi);
-  const size_t pb = dtype_bytes(g.p_dtype), gb = dtype_bytes(g.g_dtype), sb = g.state_bits == 8 ? 1 : 4;
+  const size_t pb = dtype_bytes(g.p_dtype), gb = dtype_bytes(g.g_dtype);
   for (int i = 0; i < g.count; ++i) {
     const int64_t n = g.numels[i];
     if (n < 0 || n > (int64_t)1 << 38) return fail(FM_ERR_INVALID, "group %d: bad element count at %d", gi, i);
@@ -774,33 +821,6 @@ int check_group(const fm_adamw_group& g, int gi, std::vector<Range>& ranges, std
       return fail(FM_ERR_INVALID, "group %d: misaligned tensor at %d", gi, i);
     if (g.state_bits == 8 && (!g.exp_avg_scale[i] || !g.exp_avg_sq_scale[i]))
       return fail(FM_ERR_INVALID, "group %d: null scales at %d", gi, i);
-  }
-  // `unit` bytes per element, or per block of 32 where `blocks`
-  auto add = [&](auto* list, size_t unit, bool written, bool padded, bool blocks) {
-    runs.push_back(ranges.size());
-    for (int i = 0; i < g.count; ++i) {
-      size_t n = (size_t)g.numels[i];
-      if (n == 0) continue;
-      if (padded || blocks) n = (n + 31) / 32 * (blocks ? 1 : 32);
-      const uintptr_t at = (uintptr_t)list[i];
-      ranges.push_back({at, at + n * unit, written});
-    }
-  };
-  const bool eight = g.state_bits == 8;
-  add(g.params, pb, true, false, false);
-  add(g.grads, gb, false, false, false);
-  add(g.exp_avg, sb, true, eight, false);
-  add(g.exp_avg_sq, sb, true, eight, false);
-  if (g.masters) add(g.masters, 4, true, false, false);
-  if (eight) {
-    add(g.exp_avg_scale, 1, true, false, true);
-    add(g.exp_avg_sq_scale, 1, true, false, true);
-  }
-  runs.push_back(ranges.size());
-  for (int i = 0; i < g.count; ++i) ranges.push_back({(uintptr_t)g.steps[i], (uintptr_t)g.steps[i] + 4, true});
-  if (g.lr_device) {
-    runs.push_back(ranges.size());
-    ranges.push_back({(uintptr_t)g.lr_device, (uintptr_t)g.lr_device + 4, false});
   }
   return FM_OK;
 }
@@ -963,23 +983,15 @@ struct Counts {
 };
 
 int adamw_step(const fm_adamw_group* groups, int ngroups, const float* scale, cudaStream_t stream) {
-  std::vector<Range> ranges;
   size_t tensors = 0;
-  for (int gi = 0; gi < ngroups; ++gi) tensors += groups[gi].count > 0 ? groups[gi].count : 0;
-  ranges.reserve(tensors * 8 + ngroups + 1);
-  std::vector<size_t> runs;
-  runs.reserve(ngroups * 9 + 1);
   for (int gi = 0; gi < ngroups; ++gi) {
-    const int rc = check_group(groups[gi], gi, ranges, runs);
+    const int rc = check_group(groups[gi], gi);
     if (rc != FM_OK) return rc;
+    tensors += groups[gi].count;
   }
   if (tensors == 0) return FM_OK;
   if (!aligned(scale, 4)) return fail(FM_ERR_INVALID, "misaligned gradient scale");
-  if (scale) {
-    runs.push_back(ranges.size());
-    ranges.push_back({(uintptr_t)scale, (uintptr_t)scale + 4, false});
-  }
-  int rc = check_ranges(ranges, runs);
+  int rc = check_ranges(groups, ngroups, scale);
   if (rc != FM_OK) return rc;
 
   // the kinds of the call, their elements and largest tensors

@@ -123,7 +123,7 @@ void* step_count(const at::Tensor& t, int device) {
 // A tensor that goes element by element with a parameter has its shape; the order of the elements is as
 // clear where one of the two is flat.
 void check_sizes(const at::Tensor& t, const char* name, const at::Tensor& p) {
-  REQUIRE(t.numel() == p.numel() && (t.sizes() == p.sizes() || t.dim() == 1 || p.dim() == 1),
+  REQUIRE(t.numel() == p.numel() && (p.dim() == 1 || t.dim() == 1 || t.sizes() == p.sizes()),
           "`%s` must have the parameters' sizes, or be flat", name);
 }
 
