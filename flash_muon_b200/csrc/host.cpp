@@ -456,6 +456,9 @@ PyObject* optimizer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       missing.list = nullptr;
       return list;
     }
+    // refused, if at all, before the first device steps
+    for (const Device& d : devices)
+      if (a[3] != Py_None && !d.groups.empty()) scalar(a[3], "grad_scale", d.index);
     int rc = FM_OK;
     for (Device& d : devices) {
       rc = launch(fn, d.groups, d.index, a[3]);

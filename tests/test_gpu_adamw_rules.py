@@ -129,3 +129,16 @@ def test_shapes_that_do_not_fit_are_refused():
         fm.adamw8_step([half], [z(16, 4)], *[[c] for c in codes], z(1), lr=0.1)
     scalar = z()
     fm.adamw_step([scalar], [z(1)], [z()], [z(1)], z(1), lr=0.1)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_a_factor_on_one_of_two_devices_is_refused_before_any_step():
+    ps = [torch.nn.Parameter(torch.ones(10, device=f"cuda:{i}")) for i in range(2)]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = fm.AdamW(ps)
+    opt.step()
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(AssertionError, match="`grad_scale` must be"):
+        opt.step(grad_scale=torch.ones((), device="cuda:0"))
+    assert all(torch.equal(p, b) for p, b in zip(ps, before))
