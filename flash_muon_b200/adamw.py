@@ -19,13 +19,13 @@ CPU tensors raise ``AssertionError`` like the other operators: there is no CPU p
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from collections.abc import Iterable, Sequence
 
 import torch
 from torch import Tensor
 
-from . import _host
 from ._lib import check, dtype_code, lib
 from .ops import _raw_stream
 
@@ -39,8 +39,19 @@ def _blocks(n: int) -> int:
     return -(-n // _BLOCK)
 
 
-# The entries that take lists of tensors are called through ``_host``, which checks the tensors and
-# fills the library's arrays.
+@functools.cache
+def _host():
+    """The extension through which the entries that take lists of tensors are called: it checks the tensors
+    and fills the library's arrays.  It is bound to the Python and the torch it was built for, the library is
+    not: Muon and the matrix operators run without it, so it is loaded at its first use."""
+    try:
+        from . import _host as extension
+    except ImportError as e:
+        raise ImportError("the extension flash_muon_b200._host is missing or was built for another Python or torch: "
+                          "build it with `python flash_muon_b200/build.py`") from e
+    return extension
+
+
 (_STEP, _NORM, _NORM_BYTES, _SCALE, _VALUES) = (
     ctypes.cast(fn, ctypes.c_void_p).value for fn in
     (lib.fm_adamw_step, lib.fm_grad_norm, lib.fm_grad_norm_workspace_bytes, lib.fm_scale_multi, lib.fm_adamw8_values))
@@ -59,8 +70,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     nothing is written, the counts included.  ``lr`` may be such a scalar too.  Parameters are
     bfloat16, float16 or float32; a 16-bit parameter takes gradients of its own type or float32.
     """
-    rc = _host.adamw_step(_STEP, ((params, grads, masters, exp_avgs, exp_avg_sqs, None, None, steps, None, lr, *betas,
-                                   eps, weight_decay),), grad_scale)
+    rc = _host().adamw_step(_STEP, ((params, grads, masters, exp_avgs, exp_avg_sqs, None, None, steps, None, lr,
+                                     *betas, eps, weight_decay),), grad_scale)
     if rc:
         check(rc)
 
@@ -81,8 +92,8 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Seq
     """
     if isinstance(seeds, int):
         seeds = range(seeds, seeds + len(params))
-    rc = _host.adamw_step(_STEP, ((params, grads, masters, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales,
-                                   steps, seeds, lr, *betas, eps, weight_decay),), grad_scale)
+    rc = _host().adamw_step(_STEP, ((params, grads, masters, exp_avgs, exp_avg_sqs, exp_avg_scales,
+                                     exp_avg_sq_scales, steps, seeds, lr, *betas, eps, weight_decay),), grad_scale)
     if rc:
         check(rc)
 
@@ -91,7 +102,7 @@ def adamw8_values(codes: Tensor, scales: Tensor, *, moment: int, numel: int | No
                   dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """The values that 8-bit states stand for, flat: ``moment`` 1 for ``exp_avg``, 2 for ``exp_avg_sq``;
     ``numel`` drops the padding.  bfloat16 and float32 hold them exactly."""
-    rc, values = _host.adamw8_values(_VALUES, codes, scales, moment, numel, dtype)
+    rc, values = _host().adamw8_values(_VALUES, codes, scales, moment, numel, dtype)
     if rc:
         check(rc)
     return values
@@ -118,7 +129,7 @@ def grad_norm(grads: Sequence[Tensor], max_norm: float = math.inf) -> tuple[Tens
     that clips them: two float32 scalars on the device, ready without a synchronisation for
     ``AdamW.step(grad_scale=...)``.  A norm that is not finite gives the factor NaN, with which a step
     is not taken.  Partial sums are added in 64 bits in a fixed order: equal inputs, equal bits."""
-    rc, norm, scale = _host.grad_norm(_NORM, _NORM_BYTES, grads, max_norm)
+    rc, norm, scale = _host().grad_norm(_NORM, _NORM_BYTES, grads, max_norm)
     if rc:
         check(rc)
     return norm, scale
@@ -135,7 +146,7 @@ def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float) -> T
     if not grads:
         return torch.tensor(0.0)
     norm, scale = grad_norm(grads, max_norm)
-    rc = _host.scale(_SCALE, grads, scale)
+    rc = _host().scale(_SCALE, grads, scale)
     if rc:
         check(rc)
     return norm
@@ -206,14 +217,14 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        rc = _host.optimizer_step(_STEP, self.param_groups, self.state, grad_scale)
+        rc = _host().optimizer_step(_STEP, self.param_groups, self.state, grad_scale)
         if isinstance(rc, list):  # parameters that have no state yet
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("take one step before capturing: a parameter has no state yet")
             for p, group in rc:
                 with torch.cuda.device(p.device):
                     self._init_state(p, group)
-            rc = _host.optimizer_step(_STEP, self.param_groups, self.state, grad_scale)
+            rc = _host().optimizer_step(_STEP, self.param_groups, self.state, grad_scale)
         if rc:
             check(rc)
         return loss

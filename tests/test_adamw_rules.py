@@ -2,6 +2,7 @@
 needed."""
 import shutil
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -30,3 +31,28 @@ def test_misaligned_values_are_refused(dtype, size):
         assert b"misaligned" in lib.fm_last_error()
         assert lib.fm_adamw8_encode(0x1000 + off, dtype, 32, 2, 0x2000, 0x3000, None) == INVALID
         assert b"misaligned" in lib.fm_last_error()
+
+
+def test_muon_needs_no_extension():
+    """Where the Python extension does not load the rest of the package does; what needs it names the build."""
+    code = """if True:
+        import sys
+        sys.modules["flash_muon_b200._host"] = None          # its import fails
+        import torch, flash_muon_b200 as fm
+        fm.Muon, fm.matmul_transpose, fm.fast_newtonschulz
+        assert fm.newtonschulz_workspace_bytes(4, 4) > 0
+        p = torch.nn.Parameter(torch.zeros(4, 4))
+        p.grad = torch.zeros(4, 4)
+        for call in (lambda: fm.grad_norm([p]), lambda: fm.clip_grad_norm_([p], 1.0), lambda: fm.AdamW([p]).step(),
+                     lambda: fm.adamw8_values(p, p, moment=1), lambda: fm.adamw_step([p], [p], [p], [p], p, lr=1.0),
+                     lambda: fm.adamw8_step([p], [p], [p], [p], [p], [p], p, lr=1.0)):
+            try:
+                call()
+            except ImportError as e:
+                assert "python flash_muon_b200/build.py" in str(e)
+            else:
+                raise AssertionError
+        print("fine")
+    """
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT, timeout=300)
+    assert run.stdout.strip() == "fine", run.stderr
