@@ -196,9 +196,8 @@ class AdamW(torch.optim.Optimizer):
     def _eight(self, p: Tensor, group) -> bool:
         return group["state_bits"] == 8 and p.numel() >= group["min_8bit_numel"]
 
-    def _init_state(self, p: Tensor, group) -> dict:
-        state = self.state[p]
-        state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+    def _init_state(self, p: Tensor, group) -> None:
+        state = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
         if self._eight(p, group):
             blocks = _blocks(p.numel())
             for name in ("exp_avg", "exp_avg_sq"):
@@ -209,7 +208,7 @@ class AdamW(torch.optim.Optimizer):
                 state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         if group["master_weights"] and p.dtype != torch.float32:
             state["master"] = p.detach().float().contiguous().clone()
-        return state
+        self.state[p] = state  # whole, or after an error (out of memory) not at all
 
     def step(self, closure=None, *, grad_scale: Tensor | None = None):
         """One step of every parameter that has a gradient.  ``grad_scale``: see ``adamw_step``."""

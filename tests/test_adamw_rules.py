@@ -6,7 +6,9 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
+import flash_muon_b200 as fm
 from flash_muon_b200 import _lib
 from flash_muon_b200._lib import lib
 
@@ -56,3 +58,24 @@ def test_muon_needs_no_extension():
     """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT, timeout=300)
     assert run.stdout.strip() == "fine", run.stderr
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_cannot_be_made_is_not_left_half_made(bits, monkeypatch):
+    p = torch.nn.Parameter(torch.zeros(64, dtype=torch.bfloat16))
+    opt = fm.AdamW([p], state_bits=bits, min_8bit_numel=0, master_weights=True)
+    zeros, left = torch.zeros, [2]
+
+    def failing(*args, **kwargs):
+        left[0] -= 1
+        if left[0] < 0:
+            raise torch.OutOfMemoryError("no memory")
+        return zeros(*args, **kwargs)
+
+    monkeypatch.setattr(torch, "zeros", failing)
+    with pytest.raises(torch.OutOfMemoryError):
+        opt._init_state(p, opt.param_groups[0])
+    assert p not in opt.state
+    left[0] = 100
+    opt._init_state(p, opt.param_groups[0])
+    assert {"step", "exp_avg", "exp_avg_sq", "master"} <= set(opt.state[p])
