@@ -242,28 +242,40 @@ class AdamW(torch.optim.Optimizer):
         """Loads a checkpoint of this class or of ``torch.optim.AdamW``.  Moments keep 32 bits whatever the
         parameters' type (the base class would round them to it) and are converted between 32 and 8
         bits where this optimizer's groups ask for the other."""
-        saved_groups = state_dict["param_groups"]
-        own = [g["params"] for g in self.param_groups]
-        if [len(g["params"]) for g in saved_groups] != [len(g) for g in own]:
-            raise ValueError("loaded state dict has other parameter groups")
-        for saved in saved_groups:
-            for key in ("amsgrad", "maximize"):
-                if saved.get(key):
-                    raise ValueError(f"`{key}` is not supported")
         before = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
         fresh: dict = {}
-        for group, saved in zip(self.param_groups, saved_groups):
-            for p, pid in zip(group["params"], saved["params"]):
-                if pid in state_dict["state"]:
-                    fresh[p] = self._loaded(p, group, state_dict["state"][pid])
-        super().load_state_dict({"state": {}, "param_groups": saved_groups})
-        for group, settings in zip(self.param_groups, before):
-            for key, value in settings.items():  # how states are kept is this optimizer's choice
-                if key in ("state_bits", "min_8bit_numel", "master_weights") or key not in group:
-                    group[key] = value
-            if isinstance(group["lr"], Tensor) and not group["lr"].is_cuda:
-                group["lr"] = float(group["lr"])
-        self.state.update(fresh)
+
+        def convert(_, state_dict):  # behind the caller's pre-hooks; the base class gets no state to round
+            saved_groups = state_dict["param_groups"]
+            own = [g["params"] for g in self.param_groups]
+            if [len(g["params"]) for g in saved_groups] != [len(g) for g in own]:
+                raise ValueError("loaded state dict has other parameter groups")
+            for saved in saved_groups:
+                for key in ("amsgrad", "maximize"):
+                    if saved.get(key):
+                        raise ValueError(f"`{key}` is not supported")
+            for group, saved in zip(self.param_groups, saved_groups):
+                for p, pid in zip(group["params"], saved["params"]):
+                    if pid in state_dict["state"]:
+                        fresh[p] = self._loaded(p, group, state_dict["state"][pid])
+            return {**state_dict, "state": {}}
+
+        def install(_):  # ahead of the caller's post-hooks
+            for group, settings in zip(self.param_groups, before):
+                for key, value in settings.items():  # how states are kept is this optimizer's choice
+                    if key in ("state_bits", "min_8bit_numel", "master_weights") or key not in group:
+                        group[key] = value
+                if isinstance(group["lr"], Tensor) and not group["lr"].is_cuda:
+                    group["lr"] = float(group["lr"])
+            self.state.update(fresh)
+
+        hooks = (self.register_load_state_dict_pre_hook(convert),
+                 self.register_load_state_dict_post_hook(install, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     def _loaded(self, p: Tensor, group, saved: dict) -> dict:
         for key in ("step", "exp_avg", "exp_avg_sq"):

@@ -79,3 +79,48 @@ def test_a_state_that_cannot_be_made_is_not_left_half_made(bits, monkeypatch):
     left[0] = 100
     opt._init_state(p, opt.param_groups[0])
     assert {"step", "exp_avg", "exp_avg_sq", "master"} <= set(opt.state[p])
+
+
+def checkpoint(n=5, value=0.25, cls=torch.optim.AdamW, **settings):
+    q = torch.nn.Parameter(torch.zeros(n))
+    theirs = cls([q], **settings)
+    q.grad = torch.ones(n)
+    theirs.step()
+    saved = theirs.state_dict()
+    saved["state"][0]["exp_avg"] = torch.full((n,), value)
+    return saved
+
+
+def test_load_hooks_see_and_change_the_states():
+    opt = fm.AdamW([torch.nn.Parameter(torch.zeros(5))])
+    p, seen = opt.param_groups[0]["params"][0], []
+
+    def before(o, state_dict):
+        seen.append(len(state_dict["state"]))
+        state = {k: {**v, "exp_avg": 2 * v["exp_avg"]} for k, v in state_dict["state"].items()}
+        return {**state_dict, "state": state}
+
+    def after(o):
+        seen.append((o is opt, float(o.state[p]["exp_avg"][0]), o.param_groups[0]["state_bits"]))
+
+    handles = [opt.register_load_state_dict_pre_hook(before), opt.register_load_state_dict_post_hook(after)]
+    opt.load_state_dict(checkpoint())
+    assert seen == [1, (True, 0.5, 32)] and (opt.state[p]["exp_avg"] == 0.5).all()
+    for handle in handles:
+        handle.remove()
+    opt.load_state_dict(checkpoint(value=3.0))               # nothing of the first load stays registered
+    assert (opt.state[p]["exp_avg"] == 3.0).all() and len(seen) == 2
+
+
+def test_a_refused_checkpoint_changes_nothing():
+    opt = fm.AdamW([torch.nn.Parameter(torch.zeros(5))], lr=0.5)
+    p = opt.param_groups[0]["params"][0]
+    opt.load_state_dict(checkpoint(lr=0.125))
+    keep = opt.state[p]
+    with pytest.raises(ValueError, match="size"):
+        opt.load_state_dict(checkpoint(n=6))
+    with pytest.raises(ValueError, match="maximize"):
+        opt.load_state_dict(checkpoint(maximize=True, lr=0.75))
+    assert opt.state[p] is keep and opt.param_groups[0]["lr"] == 0.125
+    opt.load_state_dict(checkpoint(value=1.0))
+    assert (opt.state[p]["exp_avg"] == 1.0).all()
