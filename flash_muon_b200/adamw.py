@@ -241,7 +241,9 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """Loads a checkpoint of this class or of ``torch.optim.AdamW``.  Moments keep 32 bits whatever the
         parameters' type (the base class would round them to it) and are converted between 32 and 8
-        bits where this optimizer's groups ask for the other."""
+        bits where this optimizer's groups ask for the other.  A learning rate that is a tensor here stays
+        that tensor and takes the checkpoint's value; else the value becomes a float.  The states are new
+        tensors: a step that was captured in a CUDA graph has to be captured again."""
         before = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
         fresh: dict = {}
 
@@ -265,7 +267,11 @@ class AdamW(torch.optim.Optimizer):
                 for key, value in settings.items():  # how states are kept is this optimizer's choice
                     if key in ("state_bits", "min_8bit_numel", "master_weights") or key not in group:
                         group[key] = value
-                if isinstance(group["lr"], Tensor) and not group["lr"].is_cuda:
+                lr = settings["lr"]
+                if isinstance(lr, Tensor):               # a schedule holds it
+                    lr.copy_(group["lr"]) if isinstance(group["lr"], Tensor) else lr.fill_(group["lr"])
+                    group["lr"] = lr
+                else:
                     group["lr"] = float(group["lr"])
             self.state.update(fresh)
 

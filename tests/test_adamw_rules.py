@@ -124,3 +124,12 @@ def test_a_refused_checkpoint_changes_nothing():
     assert opt.state[p] is keep and opt.param_groups[0]["lr"] == 0.125
     opt.load_state_dict(checkpoint(value=1.0))
     assert (opt.state[p]["exp_avg"] == 1.0).all()
+
+
+def test_a_learning_rate_on_the_device_loads_as_a_float():
+    """Where this optimizer's own is one; the checkpoint's tensor may lie anywhere."""
+    opt = fm.AdamW([torch.nn.Parameter(torch.zeros(5))], lr=0.5)
+    saved = checkpoint()
+    saved["param_groups"][0]["lr"] = torch.tensor(0.125)
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 0.125 and isinstance(opt.param_groups[0]["lr"], float)

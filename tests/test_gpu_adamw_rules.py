@@ -142,3 +142,27 @@ def test_a_factor_on_one_of_two_devices_is_refused_before_any_step():
     with pytest.raises(AssertionError, match="`grad_scale` must be"):
         opt.step(grad_scale=torch.ones((), device="cuda:0"))
     assert all(torch.equal(p, b) for p, b in zip(ps, before))
+
+
+@pytest.mark.parametrize("saved_as", ["cpu", "device", "float"])
+def test_a_learning_rate_tensor_outlives_a_checkpoint(saved_as):
+    """A schedule holds the tensor itself: it takes the loaded value and stays."""
+    p = torch.nn.Parameter(torch.zeros(5, device=DEV))
+    p.grad = torch.ones_like(p)
+    lr = torch.tensor(0.5, device=DEV)
+    opt = fm.AdamW([p], lr=lr, weight_decay=0.0)
+    opt.step()
+    saved = opt.state_dict()
+    value = {"cpu": torch.tensor(0.125), "device": torch.tensor(0.125, device=DEV), "float": 0.125}[saved_as]
+    saved["param_groups"][0]["lr"] = value
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.125
+    lr.fill_(0.25)
+    before = p.detach().clone()
+    opt.step()
+    # equal gradients: m / sqrt(v), both corrected, is 1 but for eps
+    assert torch.allclose(before - p, torch.full_like(p, 0.25), rtol=1e-4)
+    other = fm.AdamW([p], lr=0.75)
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["lr"] == 0.125 and isinstance(other.param_groups[0]["lr"], float)
+    other.step()
