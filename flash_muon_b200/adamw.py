@@ -239,7 +239,8 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------ checkpoints
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
-        """Loads a checkpoint of this class or of ``torch.optim.AdamW``.  Moments keep 32 bits whatever the
+        """Loads a checkpoint of this class or of ``torch.optim.AdamW`` (or ``Adam`` without weight decay).
+        Moments keep 32 bits whatever the
         parameters' type (the base class would round them to it) and are converted between 32 and 8
         bits where this optimizer's groups ask for the other.  A learning rate that is a tensor here stays
         that tensor and takes the checkpoint's value; else the value becomes a float.  The states are new
@@ -256,6 +257,8 @@ class AdamW(torch.optim.Optimizer):
                 for key in ("amsgrad", "maximize"):
                     if saved.get(key):
                         raise ValueError(f"`{key}` is not supported")
+                if saved.get("decoupled_weight_decay") is False and saved.get("weight_decay"):
+                    raise ValueError("a checkpoint of Adam, whose weight decay enters the gradient, is not supported")
             for group, saved in zip(self.param_groups, saved_groups):
                 for p, pid in zip(group["params"], saved["params"]):
                     if pid in state_dict["state"]:
@@ -267,6 +270,8 @@ class AdamW(torch.optim.Optimizer):
                 for key, value in settings.items():  # how states are kept is this optimizer's choice
                     if key in ("state_bits", "min_8bit_numel", "master_weights") or key not in group:
                         group[key] = value
+                if "decoupled_weight_decay" in group:
+                    group["decoupled_weight_decay"] = True  # without decay Adam is AdamW
                 lr = settings["lr"]
                 if isinstance(lr, Tensor):               # a schedule holds it
                     lr.copy_(group["lr"]) if isinstance(group["lr"], Tensor) else lr.fill_(group["lr"])

@@ -133,3 +133,18 @@ def test_a_learning_rate_on_the_device_loads_as_a_float():
     saved["param_groups"][0]["lr"] = torch.tensor(0.125)
     opt.load_state_dict(saved)
     assert opt.param_groups[0]["lr"] == 0.125 and isinstance(opt.param_groups[0]["lr"], float)
+
+
+def test_checkpoints_of_adam():
+    """Its weight decay is another; without one it is the same optimizer."""
+    opt = fm.AdamW([torch.nn.Parameter(torch.zeros(5))], lr=0.5)
+    with pytest.raises(ValueError, match="Adam"):
+        opt.load_state_dict(checkpoint(cls=torch.optim.Adam, weight_decay=0.1))
+    assert not opt.state and opt.param_groups[0]["lr"] == 0.5
+    opt.load_state_dict(checkpoint(cls=torch.optim.Adam, weight_decay=0.0))
+    assert opt.param_groups[0]["weight_decay"] == 0.0 and len(opt.state) == 1
+    opt.param_groups[0]["weight_decay"] = 0.1                # decoupled from here on: its own checkpoint loads
+    saved = opt.state_dict()
+    fm.AdamW([torch.nn.Parameter(torch.zeros(5))]).load_state_dict(saved)
+    opt.load_state_dict(checkpoint(weight_decay=0.25))
+    assert opt.param_groups[0]["weight_decay"] == 0.25
