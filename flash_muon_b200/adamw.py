@@ -187,6 +187,9 @@ class AdamW(torch.optim.Optimizer):
             beta1, beta2 = group["betas"]
             assert 0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, "betas must lie in [0, 1)"
             assert group["eps"] >= 0.0, "eps must not be negative"
+            lr = group["lr"]
+            assert not isinstance(lr, Tensor) or (lr.is_cuda and lr.dtype == torch.float32 and lr.numel() == 1), \
+                "`lr` must be a number or a float32 scalar on the parameters' CUDA device"
             for p in group["params"]:
                 dtype_code(p.dtype)
         except BaseException:

@@ -148,3 +148,14 @@ def test_checkpoints_of_adam():
     fm.AdamW([torch.nn.Parameter(torch.zeros(5))]).load_state_dict(saved)
     opt.load_state_dict(checkpoint(weight_decay=0.25))
     assert opt.param_groups[0]["weight_decay"] == 0.25
+
+
+def test_a_learning_rate_on_the_host_is_refused_at_once():
+    """As the step does, where it would come too late."""
+    new = lambda: [torch.nn.Parameter(torch.zeros(5))]  # noqa: E731
+    with pytest.raises(AssertionError, match="`lr` must be"):
+        fm.AdamW(new(), lr=torch.tensor(0.1))
+    opt = fm.AdamW(new())
+    with pytest.raises(AssertionError, match="`lr` must be"):
+        opt.add_param_group(dict(params=new(), lr=torch.tensor(0.1)))
+    assert len(opt.param_groups) == 1
