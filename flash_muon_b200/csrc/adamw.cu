@@ -958,8 +958,13 @@ struct Batch {
 // Parts of a tile with 8-bit states: what a block spends on its tensor's coefficients is shared by up to
 // 8 of them, as many as leave every SM 12 blocks (5 or 6 are resident).  67 M bf16 elements, at an earlier
 // step of the kernel: 1 part 137 us, 2 132, 4 130, 8 129, 16 no better.
+// A tile's random numbers take their upper index bits from its first element, so no tile may hold indices on both
+// sides of a multiple of 2^32: where there are that many elements tiles have 8 parts, which divide it.
+constexpr long long kBlocksPerSm = 12, kMostSms = 1024;
+static_assert((1LL << 32) % (kMaxParts * kPart8) == 0);
+static_assert((1LL << 32) / (kPart8 * kBlocksPerSm * kMostSms + 1) >= kMaxParts);
 int parts_of(long long elements) {
-  const long long parts = elements / ((long long)kPart8 * 12 * sm_count() + 1);
+  const long long parts = elements / (kPart8 * kBlocksPerSm * std::min<long long>(sm_count(), kMostSms) + 1);
   return parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : (int)parts;
 }
 
