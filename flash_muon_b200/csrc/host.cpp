@@ -15,6 +15,7 @@
 #include <cctype>
 #include <cmath>
 #include <deque>
+#include <memory>
 #include <optional>
 #include <string>
 #include <vector>
@@ -72,10 +73,17 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
-void check_place(const at::Tensor& t, const char* name, int device) {
+// One look at a tensor where all is well; what is wrong is found out apart.
+[[gnu::noinline]] void refuse_place(const at::Tensor& t, const char* name) {
   REQUIRE(t.is_cuda(), "`%s` must be CUDA tensors", name);
   REQUIRE(t.layout() == at::kStrided && t.is_contiguous(), "`%s` must be contiguous", name);
-  REQUIRE(t.get_device() == device, "`%s` must be on the parameters' device", name);
+  REQUIRE(false, "`%s` must be on the parameters' device", name);
+}
+void check_place(const at::Tensor& t, const char* name, int device) {
+  const c10::TensorImpl* const x = t.unsafeGetTensorImpl();
+  const c10::Device d = x->device();
+  if (d.type() != at::kCUDA || d.index() != device || x->layout() != at::kStrided || !x->is_contiguous())
+    refuse_place(t, name);
 }
 
 void* scalar(PyObject* o, const char* name, int device) {
@@ -96,13 +104,40 @@ void mark_written(c10::TensorImpl* t) {
   if (!t->is_inference()) t->bump_version();
 }
 
-// One parameter group of a call, in arrays that live until the call returns.
+// One parameter group of a call, in arrays that live until the call returns: those of the library and the
+// tensors that it writes.
 struct Group {
-  std::vector<int64_t> numels;
-  std::vector<void*> params, grads, masters, m, v, ms, vs, steps;
-  std::vector<uint32_t> seeds;
-  std::vector<c10::TensorImpl*> written;
   fm_adamw_group g;
+  size_t count = 0, written = 0;
+  void **params, **grads, **masters, **m, **v, **ms, **vs, **steps;
+  int64_t* numels;
+  uint32_t* seeds;
+  c10::TensorImpl** marks;
+  std::unique_ptr<void*[]> mem;
+
+  Group(const fm_adamw_group& settings, size_t most, bool master) : g(settings) {
+    const bool eight = g.state_bits == 8;
+    mem.reset(new void*[most * (8 + 7 + 2 + 1)]);
+    void** at = mem.get();
+    auto take = [&](bool there) {
+      void** const x = there ? at : nullptr;
+      if (there) at += most;
+      return x;
+    };
+    g.params = params = take(true);
+    g.grads = grads = take(true);
+    g.masters = masters = take(master);
+    g.exp_avg = m = take(true);
+    g.exp_avg_sq = v = take(true);
+    g.exp_avg_scale = ms = take(eight);
+    g.exp_avg_sq_scale = vs = take(eight);
+    steps = take(true);
+    g.steps = reinterpret_cast<float**>(steps);
+    static_assert(sizeof(int64_t) == sizeof(void*));
+    g.numels = numels = reinterpret_cast<int64_t*>(take(true));
+    g.seeds = seeds = reinterpret_cast<uint32_t*>(take(eight));
+    marks = reinterpret_cast<c10::TensorImpl**>(at);
+  }
 };
 
 // What a parameter is stepped with; master, scales may be null.
@@ -158,22 +193,25 @@ class Builder {
       REQUIRE(pd != FM_F32, "float32 parameters have no master copies");
     }
     Group& x = group(pd, gd, eight, r.master != nullptr, expected);
-    x.numels.push_back(n);
-    x.params.push_back(r.p->data_ptr());
-    x.grads.push_back(r.grad->data_ptr());
-    x.m.push_back(r.m->data_ptr());
-    x.v.push_back(r.v->data_ptr());
-    x.steps.push_back(r.step);
-    if (r.master) x.masters.push_back(r.master->data_ptr());
+    const size_t i = x.count++;
+    auto put = [&](void** list, const at::Tensor& t) {
+      list[i] = t.data_ptr();
+      x.marks[x.written++] = t.unsafeGetTensorImpl();
+    };
+    x.numels[i] = n;
+    x.grads[i] = r.grad->data_ptr();
+    put(x.params, *r.p);
+    put(x.m, *r.m);
+    put(x.v, *r.v);
+    if (r.master) put(x.masters, *r.master);
     if (eight) {
-      x.ms.push_back(r.ms->data_ptr());
-      x.vs.push_back(r.vs->data_ptr());
-      x.seeds.push_back(r.seed);
+      put(x.ms, *r.ms);
+      put(x.vs, *r.vs);
+      x.seeds[i] = r.seed;
     }
-    for (const at::Tensor* t : {r.p, r.m, r.v, r.master, r.ms, r.vs})
-      if (t) x.written.push_back(t->unsafeGetTensorImpl());
+    x.steps[i] = r.step;
     c10::TensorImpl* const count = r.count->unsafeGetTensorImpl();
-    if (count != last_count_) x.written.push_back(last_count_ = count);  // one tensor may hold them all
+    if (count != last_count_) x.marks[x.written++] = last_count_ = count;  // one tensor may hold them all
   }
 
  private:
@@ -191,24 +229,13 @@ class Builder {
   Group& group(int pd, int gd, bool eight, bool master, size_t expected) {
     for (size_t i = first_; i < out_.size(); ++i) {
       Group& x = out_[i];
-      if (x.g.p_dtype == pd && x.g.g_dtype == gd && (x.g.state_bits == 8) == eight && !x.masters.empty() == master) return x;
+      if (x.g.p_dtype == pd && x.g.g_dtype == gd && (x.g.state_bits == 8) == eight && (x.masters != nullptr) == master) return x;
     }
-    out_.emplace_back();
-    Group& x = out_.back();
-    x.g = settings_;
-    x.g.p_dtype = pd;
-    x.g.g_dtype = gd;
-    x.g.state_bits = eight ? 8 : 32;
-    for (std::vector<void*>* v : {&x.params, &x.grads, &x.m, &x.v, &x.steps}) v->reserve(expected);
-    x.numels.reserve(expected);
-    x.written.reserve(expected * (eight ? 6 : 4) + (master ? expected : 0));
-    if (master) x.masters.reserve(expected);
-    if (eight) {
-      x.ms.reserve(expected);
-      x.vs.reserve(expected);
-      x.seeds.reserve(expected);
-    }
-    return x;
+    fm_adamw_group g = settings_;
+    g.p_dtype = pd;
+    g.g_dtype = gd;
+    g.state_bits = eight ? 8 : 32;
+    return out_.emplace_back(g, expected, master);
   }
 
   std::vector<Group>& out_;
@@ -317,25 +344,14 @@ int launch(decltype(&fm_adamw_step) fn, std::vector<Group>& groups, int device, 
   std::vector<fm_adamw_group> table;
   table.reserve(groups.size());
   for (Group& x : groups) {
-    auto at = [](std::vector<void*>& p) { return p.empty() ? nullptr : p.data(); };
-    x.g.params = at(x.params);
-    x.g.grads = at(x.grads);
-    x.g.masters = at(x.masters);
-    x.g.exp_avg = at(x.m);
-    x.g.exp_avg_sq = at(x.v);
-    x.g.exp_avg_scale = at(x.ms);
-    x.g.exp_avg_sq_scale = at(x.vs);
-    x.g.steps = reinterpret_cast<float* const*>(at(x.steps));
-    x.g.numels = x.numels.data();
-    x.g.seeds = x.seeds.empty() ? nullptr : x.seeds.data();
-    x.g.count = (int32_t)x.numels.size();
+    x.g.count = (int32_t)x.count;
     table.push_back(x.g);
   }
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   const int rc = fn(table.data(), (int)table.size(), scale, c10::cuda::getCurrentCUDAStream().stream());
   if (rc == FM_OK)
     for (const Group& x : groups)
-      for (c10::TensorImpl* t : x.written) mark_written(t);
+      for (size_t i = 0; i < x.written; ++i) mark_written(x.marks[i]);
   return rc;
 }
 
