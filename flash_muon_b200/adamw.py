@@ -128,7 +128,9 @@ def grad_norm(grads: Sequence[Tensor], max_norm: float = math.inf) -> tuple[Tens
     """Euclidean norm over all elements of ``grads`` and the factor ``min(1, max_norm / (norm + 1e-6))``
     that clips them: two float32 scalars on the device, ready without a synchronisation for
     ``AdamW.step(grad_scale=...)``.  A norm that is not finite gives the factor NaN, with which a step
-    is not taken.  Partial sums are added in 64 bits in a fixed order: equal inputs, equal bits."""
+    is not taken.  Squares are formed in float32: one element above 1.8e19 makes the norm infinite, and elements
+    below 1e-23 count for nothing.  Partial sums are added in 64 bits in a fixed order: equal inputs, equal
+    bits."""
     rc, norm, scale = _host().grad_norm(_NORM, _NORM_BYTES, grads, max_norm)
     if rc:
         check(rc)
@@ -138,8 +140,10 @@ def grad_norm(grads: Sequence[Tensor], max_norm: float = math.inf) -> tuple[Tens
 def clip_grad_norm_(parameters: Tensor | Iterable[Tensor], max_norm: float) -> Tensor:
     """Scales the gradients of ``parameters`` in place so that their norm is at most ``max_norm`` and
     returns the norm they had (``torch.nn.utils.clip_grad_norm_`` for the Euclidean norm).  Gradients
-    within the norm are read once and left alone; if the norm is not finite all become NaN.  A parameter
-    that is given twice is refused."""
+    within the norm are read once and left alone; if the norm is not finite (an element above 1.8e19 makes it
+    infinite) all become NaN.  What torch's function does beyond that is not there: other norms,
+    ``error_if_nonfinite``, gradients on several devices, gradients that are not contiguous (channels-last
+    ones); a parameter that is given twice is refused."""
     if isinstance(parameters, Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
@@ -243,11 +247,11 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
         """Loads a checkpoint of this class or of ``torch.optim.AdamW`` (or ``Adam`` without weight decay).
-        Moments keep 32 bits whatever the
-        parameters' type (the base class would round them to it) and are converted between 32 and 8
-        bits where this optimizer's groups ask for the other.  A learning rate that is a tensor here stays
-        that tensor and takes the checkpoint's value; else the value becomes a float.  The states are new
-        tensors: a step that was captured in a CUDA graph has to be captured again."""
+        Moments keep 32 bits whatever the parameters' type (the base class would round them to it) and are
+        converted between 32 and 8 bits where this optimizer's groups ask for the other.  A learning rate
+        that is a tensor here stays that tensor and takes the checkpoint's value; else the value becomes a
+        float.  The states are new tensors: a step that was captured in a CUDA graph has to be captured
+        again."""
         before = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
         fresh: dict = {}
 

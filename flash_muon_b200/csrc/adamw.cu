@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(kWhole ? kMaxThreads : kThreads) adamw_kernel(
 //   encode: scaled by the block's power of two (state8.cuh) the code is the bits above bit 20, the
 //   random number is added below and cut off.
 // The parts of a block's tile are copied to shared memory two ahead.  67 M bf16 elements 115 us (5.9 TB/s,
-// 90 % of a copy; 46 instructions per element, issue slots 79 % busy), f32 169 us (98 %), bf16 with masters 172 us
-// (96 %); elements at odd addresses 199 to 279 us.
+// 90 % of a copy; 46 instructions per element, issue slots 77 % busy), f32 169 us (98 %), bf16 with masters 173 us
+// (96 %); elements at odd addresses 209 to 287 us (48 to 66 %).
 // Two cases that hardly ever occur leave this path: a block whose largest magnitude is not finite or
 // beyond what one normal fp32 factor scales, and a positive v whose code came out 0.
 typedef unsigned long long f32x2;
@@ -395,7 +395,8 @@ struct Staged {
 };
 
 // Resident blocks per SM that registers are kept down for: 6, with two float32 arrays in shared memory 5.
-// A seventh of 16-bit types leaves 72 registers, which some builds spill (114 to 132 us where 6 take 115).
+// A seventh of 16-bit types leaves 72 registers, which some builds spill (114 to 132 us where 6 take 115).  16-bit
+// parameters with masters and float32 gradients spill 8 bytes at 5: 67 M elements 196 us, 95 % of a copy.
 template <typename W, typename G>
 constexpr int resident8() {
   return sizeof(W) + sizeof(G) <= 6 ? 6 : 5;

@@ -21,11 +21,12 @@ constexpr int kSmallTable = 64;      // tensors of one launch: the table travels
 constexpr int kLargeTable = 1024;
 // Up to 256 units of 1024 elements, a unit per warp at a time, go to one cluster of blocks, which adds up
 // in shared memory and leaves the result itself: one launch instead of two, 2 us less host time.  On the device
-// that is 2.2 us instead of 3.1 for 2^16 bf16 elements, 3.1 instead of 3.2 for 2^18, 4.1 instead of 3.2 for 2^19.
+// that is 2.5 us instead of 3.0 for 2^16 bf16 elements, 2.8 instead of 3.2 for 2^17, 3.6 instead of 3.3 for 2^18,
+// 5.4 instead of 3.4 for 2^19.
 constexpr int kUnit = 1024, kMaxUnits = 256, kCluster = 8, kClusterThreads = 512;
 // Scaling walks with up to 128 blocks per SM.  A block per tile would be faster where there is something
 // to do (353 M bf16 elements: 209 instead of 222 us), but within the norm, as most steps are, its
-// 172,000 blocks take 93 us to find that out, these 13.
+// 172,000 blocks take 93 us to find that out, these 13 to 18.
 constexpr int kScaleThreads = 128, kScaleTile = 2048, kScaleBlocks = 128;
 constexpr int kMaxBlocks = 1184;     // partial sums of one launch, 8 per SM; fixed, so that the
                                      // order of the sum is the same whatever else runs
@@ -85,7 +86,7 @@ __device__ __forceinline__ void walk(const Tab& tab, int chunk, Body body) {
   }
 }
 
-// Sum of squares of a chunk: 32 to 36 squares per thread in fp32.
+// Sum of squares of a chunk: at most 32 squares per thread in fp32.
 template <typename T>
 __device__ __forceinline__ float chunk_sumsq(const T* g, int len) {
   constexpr int V = 16 / sizeof(T);
@@ -168,7 +169,7 @@ __device__ __forceinline__ float unit_sumsq(const T* g, int len) {
   return s;
 }
 
-// Bound by latency: 97 vectors of 1024 in one launch, 8.2 us a call with its host side (two launches 10.7).
+// Bound by latency: 97 vectors of 1024 in one launch, 8.4 to 9.1 us a call with its host side (two launches 10.7).
 template <int N>
 __global__ void __cluster_dims__(kCluster) __launch_bounds__(kClusterThreads)
 grad_norm_small_kernel(const __grid_constant__ Table<N> tab, double max_norm, float* result) {

@@ -1,6 +1,6 @@
 // Python side of the multi-tensor entry points: checks lists of tensors and turns them into the C
-// ABI's arrays.  A call over 65 tensors and four lists makes 1500 attribute look-ups, 100 us in
-// Python against 6 us on the GPU; here they take 4 us.
+// ABI's arrays, and marks what is written for autograd.  A call over 65 tensors and four lists makes 1500
+// attribute look-ups, 100 us in Python against 6 us on the GPU; here they take 6 us, the marks included.
 // The C entries are given by address, so this module is bound to no particular shared library.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
