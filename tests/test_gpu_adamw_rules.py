@@ -166,3 +166,30 @@ def test_a_learning_rate_tensor_outlives_a_checkpoint(saved_as):
     other.load_state_dict(saved)
     assert other.param_groups[0]["lr"] == 0.125 and isinstance(other.param_groups[0]["lr"], float)
     other.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipping_and_steps_in_two_graphs(bits):
+    """Graphs captured apart share no scratch, and each replay clips the gradients that are there."""
+    ps = [torch.nn.Parameter(torch.randn(n, device=DEV)) for n in (300, 50000, 0, 8)]
+    for p in ps:
+        p.grad = torch.randn_like(p)
+    opt = fm.AdamW(ps, lr=0.01, state_bits=bits, min_8bit_numel=0)
+    opt.step()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norm = fm.clip_grad_norm_(ps, 1.0)
+            opt.step()
+        graphs.append((graph, norm))
+    for i in range(6):
+        for p in ps:
+            p.grad.normal_()
+        want = sum(float(p.grad.double().square().sum()) for p in ps) ** 0.5
+        graph, norm = graphs[i % 2]
+        graph.replay()
+        # 17 u for the norm; the factor and the products of the clipped elements 5 u more
+        assert abs(float(norm) / want - 1) <= 17 * 2.0 ** -24
+        assert abs(sum(float(p.grad.double().square().sum()) for p in ps) ** 0.5 - 1) <= 24 * 2.0 ** -24 + 1e-6 / want
+    assert all(float(opt.state[p]["step"]) == 7.0 for p in ps)
