@@ -768,6 +768,7 @@ int check_ranges(const fm_adamw_group* groups, int ngroups, const float* scale) 
   std::vector<Range> r;
   r.reserve(total);
   if (scale) r.push_back({(uintptr_t)scale, (uintptr_t)scale + 4, false});
+  std::vector<size_t> runs = {0, r.size()};  // where the sorted lists begin, and the end
   for (int gi = 0; gi < ngroups; ++gi) {
     if (groups[gi].count == 0) continue;
     for_lists(groups[gi], [&](int count, bool, auto at) {
@@ -777,9 +778,13 @@ int check_ranges(const fm_adamw_group* groups, int ngroups, const float* scale) 
         if (x.begin != x.end) r.push_back(x);
       }
       if (!std::is_sorted(r.begin() + from, r.end(), less)) std::sort(r.begin() + from, r.end(), less);
-      std::inplace_merge(r.begin(), r.begin() + from, r.end(), less);
+      runs.push_back(r.size());
     });
   }
+  for (size_t step = 1; step + 1 < runs.size(); step *= 2)  // runs[i] .. runs[i + step] is in order
+    for (size_t i = 0; i + step + 1 < runs.size(); i += 2 * step)
+      std::inplace_merge(r.begin() + runs[i], r.begin() + runs[i + step],
+                         r.begin() + runs[std::min(i + 2 * step, runs.size() - 1)], less);
   uintptr_t any = 0, written = 0;
   for (const Range& x : r) {
     if (x.begin < (x.written ? any : written)) return fail(FM_ERR_INVALID, "tensors of the step overlap (the same parameter twice?)");
